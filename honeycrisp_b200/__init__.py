@@ -7,12 +7,12 @@ Public surface:
   shardBatch, columnBlock, batchedMatmulSharded, matmulColumnSplit - honeycrisp_b200.sharding
 The compute library is honeycrisp_b200/libhccuda.so (C ABI in include/hc_cuda.h).
 """
-from .backend import (AllocationFailed, BackendError, CUDABackend, CUDAData, DeviceTimeout, DType,
+from .backend import (AdamWPlan, AllocationFailed, BackendError, CUDABackend, CUDAData, DeviceTimeout, DType,
                       KernelFailed, NotImplementedByBackend)
 from .linalg import Tensor, batchedMatmul, matmul
 from .linear import Linear
 
 __all__ = [
-    "AllocationFailed", "BackendError", "CUDABackend", "CUDAData", "DeviceTimeout", "DType", "KernelFailed",
+    "AdamWPlan", "AllocationFailed", "BackendError", "CUDABackend", "CUDAData", "DeviceTimeout", "DType", "KernelFailed",
     "Linear", "NotImplementedByBackend", "Tensor", "batchedMatmul", "matmul",
 ]

@@ -39,6 +39,18 @@ class LaunchInfo(ctypes.Structure):
     ]
 
 
+HC_ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+class Epilogue(ctypes.Structure):
+    _fields_ = [("activation", _int), ("bias", _vp), ("residual", _vp), ("pre", _vp), ("grad_pre", _vp)]
+
+
+class AdamWTensor(ctypes.Structure):
+    _fields_ = [("param", _vp), ("grad", _vp), ("moment1", _vp), ("moment2", _vp), ("param_copy", _vp), ("count", _i64),
+                ("param_dtype", _int), ("grad_dtype", _int)]
+
+
 class PlanInfo(ctypes.Structure):
     _fields_ = [
         ("tile_m", _int), ("tile_n", _int), ("ctas_per_tile", _int), ("slabs_per_slot", _int),
@@ -73,6 +85,14 @@ SIGNATURES = {
     "hc_host_sync": (_int, [_vp]),
     "hc_matmul_colblock": (_int, [_vp, _int, _int, _vp, _int, _vp, _int, _int, _i64, _i64, _i64, _i64, _i64, _vp]),
     "hc_linear_forward": (_int, [_vp, _int, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "hc_matmul_epilogue": (_int, [_vp, _int, _vp, _int, _vp, _int, _i64, _i64, _i64, ctypes.POINTER(Epilogue), _vp]),
+    "hc_activation_grad": (_int, [_vp, _int, _int, _vp, _vp, _i64, _i64, _vp, _vp]),
+    "hc_layer_norm": (_int, [_vp, _int, _int, _vp, _vp, _vp, _i64, _i64, ctypes.c_float, _vp, _vp, _vp]),
+    "hc_layer_norm_grad": (_int, [_vp, _int, _int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp]),
+    "hc_grouped_matmul": (_int, [_vp, _int, _i64, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp]),
+    "hc_grouped_matmul_weight_grad": (_int, [_vp, _int, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "hc_adamw": (_int, [_vp, ctypes.POINTER(AdamWTensor), _i64, _i64, ctypes.c_double, ctypes.c_double, ctypes.c_double,
+                        ctypes.c_double, ctypes.c_double]),
     "hc_column_sum": (_int, [_vp, _int, _vp, _i64, _i64, _vp]),
     "hc_cast": (_int, [_vp, _int, _int, _vp, _i64, _vp]),
     "hc_add": (_int, [_vp, _int, _vp, _vp, _i64, _vp]),

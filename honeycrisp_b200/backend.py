@@ -76,6 +76,18 @@ def _as_dtype(dtype) -> DType:
     return dt
 
 
+_TORCH_DTYPE = {}
+
+
+def _torch_dtype(t) -> Optional[DType]:
+    """The DType of a torch dtype; None where the framework has none (bfloat16, for one)."""
+    try:
+        return _TORCH_DTYPE[t]
+    except KeyError:
+        name = str(t).replace("torch.", "")
+        return _TORCH_DTYPE.setdefault(t, DType(name) if name in DType._value2member_map_ else None)
+
+
 _HC_DTYPE = {DType.float16: L.HC_F16, DType.float32: L.HC_F32}
 
 
@@ -237,6 +249,51 @@ class CUDAData:
             self.free()
         except Exception:
             pass
+
+
+class AdamWPlan:
+    """The tensors of an AdamW step, laid out once for all steps (Adam of the reference's Optimizer.swift holds
+    its parameters the same way).  Parameters and gradients are float16 or float32, moments float32; torch tensors
+    bring their type and length, CUDAData needs `dtype` (and `gradDType`, if it differs) and `count` in its dict.  The plan keeps
+    the tensors alive; their addresses must stay what they are."""
+
+    def __init__(self, backend: "CUDABackend", tensors):
+        tensors = list(tensors)
+        self.count = len(tensors)
+        self._table = (L.AdamWTensor * max(1, self.count))()
+        self._keep, self._updated = [], []
+        for row, t in zip(self._table, tensors):
+            if set(t) - {"param", "grad", "moment1", "moment2", "copy", "count", "dtype", "gradDType"}:
+                raise ValueError(f"AdamWPlan: unknown entries {sorted(t)}")
+            p = t["param"]
+            count = int(t["count"]) if t.get("count") is not None else p.numel()
+            pd = self._dtype(p, t.get("dtype"))
+            gd = self._dtype(t["grad"], t.get("gradDType", t.get("dtype")))
+            if pd not in _HC_DTYPE or gd not in _HC_DTYPE:
+                raise NotImplementedByBackend(f"AdamW for dtypes {pd.value}, {gd.value}")
+            fields = [("param", p, pd), ("grad", t["grad"], gd), ("moment1", t["moment1"], DType.float32),
+                      ("moment2", t["moment2"], DType.float32), ("param_copy", t.get("copy"), DType.float16)]
+            for name, x, dt in fields:
+                if isinstance(x, np.ndarray):
+                    raise TypeError(f"AdamWPlan: {name} must lie on the device")
+                ptr, keep = backend._input(x, dt, count, name)
+                setattr(row, name, ptr or None)
+                self._keep.append(keep)
+                if name != "grad" and isinstance(x, CUDAData):
+                    self._updated.append(x)
+            row.count = count
+            row.param_dtype, row.grad_dtype = _HC_DTYPE[pd], _HC_DTYPE[gd]
+
+    @staticmethod
+    def _dtype(x, given) -> DType:
+        if given is not None and isinstance(x, CUDAData):
+            return _as_dtype(given)
+        if hasattr(x, "element_size"):
+            dt = _torch_dtype(x.dtype)
+            if dt is None:
+                raise NotImplementedByBackend(f"AdamW for dtype {x.dtype}")
+            return dt
+        raise ValueError("AdamWPlan: a CUDAData needs its dtype")
 
 
 class CUDABackend:
@@ -512,6 +569,174 @@ class CUDABackend:
         out._mark()
         out._inputs = (x_d, w_d, b_d)
         return out
+
+    # -- a feed-forward block ----------------------------------------------------------------
+    # Tensors of these calls are device buffers (CUDAData), contiguous CUDA torch tensors, or, for inputs,
+    # numpy arrays, which are staged.  Sizes are checked here; what the library refuses (overlaps, misaligned
+    # addresses, unknown activations, ranges of the scalars) raises ValueError.
+
+    def _float_dtype(self, dtype, what: str):
+        dt = _as_dtype(dtype)
+        hdt = _HC_DTYPE.get(dt)
+        if hdt is None:
+            raise NotImplementedByBackend(f"{what} for dtype {dt.value}")
+        return dt, hdt
+
+    def _input(self, x, dt: DType, count: int, what: str):
+        """(address, object to keep alive) of an input of `count` elements; None stays null."""
+        if x is None:
+            return None, None
+        if not isinstance(x, (CUDAData, np.ndarray)) and hasattr(x, "element_size"):
+            if _torch_dtype(x.dtype) is not dt:
+                raise ValueError(f"{what} has type {x.dtype}, not {dt.value}")
+            if x.device.index != self.device:
+                raise ValueError(f"{what} lies on {x.device}, the backend on device {self.device}")
+        elif isinstance(x, np.ndarray) and x.dtype != dt.numpy:
+            raise ValueError(f"{what} has type {x.dtype}, not {dt.value}")
+        ptr, n, keep = self._operand(x, dt)
+        if n < count * dt.byteSize:
+            raise ValueError(f"{what} is smaller than its {count} elements")
+        return ptr, keep
+
+    def _result(self, x, dt: DType, count: int, what: str):
+        """(address, the result itself): `x`, or a fresh buffer where it is None."""
+        if x is None:
+            x = self.allocate(count * dt.byteSize)
+        elif isinstance(x, np.ndarray):
+            raise TypeError(f"{what} must lie on the device")
+        ptr, _ = self._input(x, dt, count, what)
+        return ptr, x
+
+    def _done(self, results, inputs, mark: bool):
+        for r in results:
+            if isinstance(r, CUDAData):
+                if mark:
+                    r._mark()
+                r._inputs = inputs   # keep operands alive until the result is collected
+
+    def _activation(self, name) -> int:
+        try:
+            return L.HC_ACTIVATIONS[name or "none"]
+        except KeyError:
+            raise ValueError(f"unknown activation {name!r}; one of {sorted(L.HC_ACTIVATIONS)}") from None
+
+    def matmulEpilogue(self, a, transA: bool, b, transB: bool, rows: int, inner: int, cols: int, dtype, activation=None,
+                       bias=None, residual=None, pre=None, gradPre=None, out=None, mark: bool = True):
+        """activation(op(a) op(b) + bias) + residual, in one product, rounded once; `pre`, a device buffer, receives the
+        activation's input.  With `gradPre`: (op(a) op(b)) * activation'(gradPre), the gradient form.  `bias` has
+        `cols` elements, the other tensors rows x cols, all of `dtype`.  Returns `out`."""
+        dt, hdt = self._float_dtype(dtype, "matmul")
+        n = rows * cols
+        a_p, a_k = self._input(a, dt, rows * inner, "operand a")
+        b_p, b_k = self._input(b, dt, inner * cols, "operand b")
+        bias_p, bias_k = self._input(bias, dt, cols, "bias")
+        res_p, res_k = self._input(residual, dt, n, "residual")
+        grad_p, grad_k = self._input(gradPre, dt, n, "gradPre")
+        pre_p = self._result(pre, dt, n, "pre")[0] if pre is not None else None
+        act = self._activation(activation)
+        out_p, out = self._result(out, dt, n, "out")
+        ep = L.Epilogue(act, bias_p, res_p, pre_p, grad_p)
+        self._check(self._lib.hc_matmul_epilogue(self._ctx, hdt, a_p, 1 if transA else 0, b_p, 1 if transB else 0, rows, inner,
+                                                 cols, ctypes.byref(ep), out_p))
+        self._done((out, pre), (a_k, b_k, bias_k, res_k, grad_k), mark)
+        return out
+
+    def activationGrad(self, grad, pre, rows: int, cols: int, dtype, activation, out=None, biasGrad=True, mark: bool = True):
+        """grad * activation'(pre), and its sum over the rows in float32 (a bias's gradient), unless `biasGrad` is False or
+        None; `biasGrad` may be the buffer that receives it.  Returns (out, biasGrad)."""
+        dt, hdt = self._float_dtype(dtype, "activationGrad")
+        g_p, g_k = self._input(grad, dt, rows * cols, "grad")
+        z_p, z_k = self._input(pre, dt, rows * cols, "pre")
+        act = self._activation(activation)
+        out_p, out = self._result(out, dt, rows * cols, "out")
+        bg_p = None
+        if biasGrad is None or biasGrad is False:
+            biasGrad = None
+        else:
+            bg_p, biasGrad = self._result(None if biasGrad is True else biasGrad, DType.float32, cols, "biasGrad")
+        self._check(self._lib.hc_activation_grad(self._ctx, hdt, act, g_p, z_p, rows, cols, out_p, bg_p))
+        self._done((out, biasGrad), (g_k, z_k), mark)
+        return out, biasGrad
+
+    def layerNorm(self, x, weight, bias, rows: int, cols: int, dtype, epsilon: float = 1e-5, paramDType=DType.float32, out=None,
+                  mean=None, rstd=None, mark: bool = True):
+        """Layer normalisation of x[rows,cols] over its columns; `weight` and `bias` may be None.  `mean` and `rstd` are
+        float32 buffers of `rows` elements that receive what layerNormGrad needs, or None.  Returns `out`."""
+        dt, hdt = self._float_dtype(dtype, "layerNorm")
+        pt, hpt = self._float_dtype(paramDType, "layerNorm parameters")
+        x_p, x_k = self._input(x, dt, rows * cols, "x")
+        w_p, w_k = self._input(weight, pt, cols, "weight")
+        b_p, b_k = self._input(bias, pt, cols, "bias")
+        m_p = self._result(mean, DType.float32, rows, "mean")[0] if mean is not None else None
+        r_p = self._result(rstd, DType.float32, rows, "rstd")[0] if rstd is not None else None
+        out_p, out = self._result(out, dt, rows * cols, "out")
+        self._check(self._lib.hc_layer_norm(self._ctx, hdt, hpt, x_p, w_p, b_p, rows, cols, epsilon, out_p, m_p, r_p))
+        self._done((out, mean, rstd), (x_k, w_k, b_k), mark)
+        return out
+
+    def layerNormGrad(self, grad, x, weight, mean, rstd, rows: int, cols: int, dtype, paramDType=DType.float32, out=None,
+                      weightGrad=True, biasGrad=True, mark: bool = True):
+        """Backward of layerNorm: (dx, weightGrad, biasGrad).  `out` False leaves dx out; the parameters' gradients are
+        written, not accumulated: True for a fresh buffer, a buffer, or None / False for none."""
+        dt, hdt = self._float_dtype(dtype, "layerNormGrad")
+        pt, hpt = self._float_dtype(paramDType, "layerNorm parameters")
+        g_p, g_k = self._input(grad, dt, rows * cols, "grad")
+        x_p, x_k = self._input(x, dt, rows * cols, "x")
+        w_p, w_k = self._input(weight, pt, cols, "weight")
+        m_p, m_k = self._input(mean, DType.float32, rows, "mean")
+        r_p, r_k = self._input(rstd, DType.float32, rows, "rstd")
+
+        def wanted(v, t, n, what):
+            if v is None or v is False:
+                return None, None
+            return self._result(None if v is True else v, t, n, what)
+
+        dx_p, dx = wanted(True if out is None else out, dt, rows * cols, "out")
+        dw_p, dw = wanted(weightGrad, pt, cols, "weightGrad")
+        db_p, db = wanted(biasGrad, pt, cols, "biasGrad")
+        self._check(self._lib.hc_layer_norm_grad(self._ctx, hdt, hpt, g_p, x_p, w_p, m_p, r_p, rows, cols, dx_p, dw_p, db_p))
+        self._done((dx, dw, db), (g_k, x_k, w_k, m_k, r_k), mark)
+        return dx, dw, db
+
+    def groupedMatmul(self, groupCount: int, offsets, a, b, transB: bool, totalRows: int, inner: int, cols: int, dtype, out=None,
+                      mark: bool = True):
+        """out[r] = a[r] op(b[g]) for offsets[g] <= r < offsets[g + 1]: products grouped by expert.  `offsets` is int64, ascending,
+        groupCount + 1 long, and read on the device when the call runs; rows of `out` outside the groups keep
+        what they hold (a fresh `out` holds anything there)."""
+        dt, hdt = self._float_dtype(dtype, "groupedMatmul")
+        o_p, o_k = self._input(offsets, DType.int64, groupCount + 1, "offsets")
+        a_p, a_k = self._input(a, dt, totalRows * inner, "operand a")
+        b_p, b_k = self._input(b, dt, groupCount * inner * cols, "operand b")
+        out_p, out = self._result(out, dt, totalRows * cols, "out")
+        self._check(self._lib.hc_grouped_matmul(self._ctx, hdt, groupCount, o_p, a_p, b_p, 1 if transB else 0, totalRows, inner, cols,
+                                                out_p))
+        self._done((out,), (o_k, a_k, b_k), mark)
+        return out
+
+    def groupedMatmulWeightGrad(self, groupCount: int, offsets, a, b, totalRows: int, rows: int, cols: int, dtype, out=None,
+                                mark: bool = True):
+        """out[g] = a_g^T b_g over each group's rows of a[totalRows,rows] and b[totalRows,cols]; zeros for an empty group."""
+        dt, hdt = self._float_dtype(dtype, "groupedMatmul")
+        o_p, o_k = self._input(offsets, DType.int64, groupCount + 1, "offsets")
+        a_p, a_k = self._input(a, dt, totalRows * rows, "operand a")
+        b_p, b_k = self._input(b, dt, totalRows * cols, "operand b")
+        out_p, out = self._result(out, dt, groupCount * rows * cols, "out")
+        self._check(self._lib.hc_grouped_matmul_weight_grad(self._ctx, hdt, groupCount, o_p, a_p, b_p, totalRows, rows, cols, out_p))
+        self._done((out,), (o_k, a_k, b_k), mark)
+        return out
+
+    def adamWPlan(self, tensors) -> "AdamWPlan":
+        """The table of an AdamW step: a sequence of dicts with `param`, `grad`, `moment1`, `moment2` and, optionally, `copy`
+        (float16) and `count`; see AdamWPlan."""
+        return AdamWPlan(self, tensors)
+
+    def adamW(self, plan: "AdamWPlan", step: int, learningRate: float = 1e-3, beta1: float = 0.9, beta2: float = 0.999,
+              epsilon: float = 1e-8, weightDecay: float = 0.01, mark: bool = True) -> None:
+        """One AdamW step over the plan's tensors, in place; `step` counts from 1."""
+        self._check(self._lib.hc_adamw(self._ctx, plan._table, plan.count, step, learningRate, beta1, beta2, epsilon, weightDecay))
+        if mark:
+            for t in plan._updated:
+                t._mark()
 
     def columnSum(self, x, rows: int, cols: int, dtype) -> CUDAData:
         """Sum over the rows of x[rows,cols] (reduce(.sum) over the leading axis, Backend.swift:524-531)."""

@@ -9,6 +9,18 @@
 
 namespace hc {
 
+// The extras of one launch, as the kernels take them.  `aux` is the residual (added behind the
+// activation) or, in the gradient form, the pre-activation whose slope scales the product; both are
+// laid out like the result.
+struct FusedEpilogue {
+  const void* bias = nullptr;   // [N], or null
+  const void* aux = nullptr;    // residual or grad_pre, or null
+  void* pre = nullptr;          // receives z, or null
+  int act = 0;
+  int grad = 0;                 // aux is grad_pre
+  int vec = 0;                  // aux, pre and the result's pitch allow 16-byte accesses
+};
+
 // A matrix product after the reference's three flags have been folded away.
 //
 // Backend.matmul computes transOut(op(a)*op(b)) (Sources/Honeycrisp/Backend.swift:650-658).
@@ -30,6 +42,9 @@ struct GemmProblem {
   // Optional row vector of N elements (same dtype) added to every row of the product after it has
   // been rounded to the output dtype: the `h + bias` of Linear (Trainable.swift:539-544).
   const void* bias = nullptr;
+  // The epilogue applies `fe` to the unrounded product (then `bias` above is unused).
+  bool fused = false;
+  FusedEpilogue fe;
   // The contraction may not be cut into parts (which needs a float32 work area of
   // parts x batch x M x N): set by callers whose work area has a fixed size.
   bool no_split = false;
@@ -83,6 +98,8 @@ cudaError_t launch_tc(const GemmProblem& p, cudaStream_t stream, unsigned int* s
                       void* const* extra_out = nullptr, int n_extra = 0, TcCache* cache = nullptr,
                       size_t* scratch_needed = nullptr, bool private_stream = false);
 bool tc_supported(const GemmProblem& p);
+// Another kernel has been launched on `stream`: the next product waits for it before it reads anything.
+void tc_forget_predecessor(cudaStream_t stream);
 // One-thread kernel whose bounded wait is made to expire after `limit_ns` (self-test).
 cudaError_t launch_wait_probe(cudaStream_t stream, unsigned int* status_word, unsigned long long limit_ns);
 size_t tc_scratch_bytes(const GemmProblem& p, int sm_count);
@@ -90,6 +107,23 @@ size_t tc_scratch_bytes(const GemmProblem& p, int sm_count);
 struct PlanSummary { int tile_m, tile_n, ctas, slabs, parts, slots_per_part; int64_t tiles; size_t ws_bytes; };
 PlanSummary tc_describe_plan(const GemmProblem& p, int sm_count);
 
+}  // namespace hc
+
+// Products grouped by expert (csrc/gemm_grouped.cu).  Forward: a [total_rows, inner], b [groups] of
+// [inner, cols] or, trans_b, [cols, inner], out [total_rows, cols].  Weight gradient: a [total_rows, rows],
+// b [total_rows, cols], out [groups][rows, cols].  At least one group and one row; the work area and
+// `scratch_needed` as in launch_tc.
+namespace hc {
+struct GroupedProblem {
+  hc_dtype dtype;
+  bool weight_grad, trans_b;
+  int64_t groups, total_rows, rows, inner, cols;
+  const int64_t* offsets;   // device, groups + 1
+  const void *a, *b;
+  void* out;
+};
+cudaError_t launch_grouped(const GroupedProblem& p, cudaStream_t stream, unsigned int* status_word, void* scratch,
+                           size_t scratch_bytes, int sm_count, LaunchRecord* rec, size_t* scratch_needed);
 }  // namespace hc
 
 // Elementwise and reduction helpers around a Linear product (csrc/linear_ops.cu).
@@ -105,10 +139,47 @@ cudaError_t launch_random(int normal, hc_dtype dtype, unsigned long long seed, u
                           int64_t count, void* out, cudaStream_t stream);
 }  // namespace hc
 
+// The operators around a feed-forward block's products (csrc/activation.cu, norm.cu, adamw.cu).
+namespace hc {
+// Rows cut into runs for sums over them: about as many CTAs as the device holds, by the shape alone.
+struct RunSplit { int64_t strips, rows_per_run, runs; };
+RunSplit split_runs(int64_t rows, int64_t cols, int cols_per_cta);
+// out0[c] (and out1[c], from the second stack) = sum over runs of partial[run][c]
+cudaError_t launch_sum_runs(const float* partial, int64_t runs, int64_t cols, void* out0, void* out1, bool half, cudaStream_t stream);
+size_t activation_grad_scratch(hc_dtype dtype, int64_t rows, int64_t cols);
+cudaError_t launch_activation_grad(hc_dtype dtype, int act, const void* grad, const void* pre, int64_t rows, int64_t cols,
+                                   void* dpre, float* bias_grad, float* scratch, cudaStream_t stream);
+cudaError_t launch_layer_norm(hc_dtype dtype, hc_dtype param_dtype, const void* x, const void* w, const void* b, int64_t rows,
+                              int64_t cols, float epsilon, void* out, float* mean, float* rstd, cudaStream_t stream);
+size_t layer_norm_grad_scratch(hc_dtype dtype, int64_t rows, int64_t cols);
+cudaError_t launch_layer_norm_grad(hc_dtype dtype, hc_dtype param_dtype, const void* grad, const void* x, const void* w,
+                                   const float* mean, const float* rstd, int64_t rows, int64_t cols, void* dx, void* dw, void* db,
+                                   float* scratch, int* launches, cudaStream_t stream);
+struct AdamWFactors { float lr, beta1, one_minus_beta1, beta2, one_minus_beta2, epsilon, decay, inv_c1, inv_c2; };
+cudaError_t launch_adamw(const hc_adamw_tensor* tensors, int64_t count, const AdamWFactors& f, int* launches, cudaStream_t stream);
+}  // namespace hc
+
 // Context internals shared between translation units (defined in hc_api.cu).
 #include <mutex>
 namespace hc {
 std::mutex& ctx_mutex(hc_ctx* ctx);
+// A product through the usual choice of kernel; the caller holds the mutex, the device is current.
+hc_status ctx_run_problem(hc_ctx* ctx, const GemmProblem& p, int64_t flops);
+// The context's work area, grown to `bytes`: used in the order of the context's stream only.
+hc_status ctx_scratch(hc_ctx* ctx, size_t bytes, void** ptr);
+hc_status ctx_cuda_fail(hc_ctx* ctx, cudaError_t e, const char* what);
+struct DeviceGuard {
+  int prev = -1;
+  bool ok = true;
+  explicit DeviceGuard(int dev) {
+    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+    if (prev != dev) ok = (cudaSetDevice(dev) == cudaSuccess);
+  }
+  ~DeviceGuard() {
+    int cur = -1;
+    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
+  }
+};
 cudaStream_t ctx_stream(hc_ctx* ctx);
 unsigned int* ctx_status_word(hc_ctx* ctx);
 int ctx_sm_count(hc_ctx* ctx);

@@ -14,6 +14,7 @@
 // 8 through shared memory.  Each output is accumulated by exactly one thread in ascending k,
 // which is what makes the EXACT claim hold for any tile decomposition.
 #include "common.cuh"
+#include "epilogue.cuh"
 
 namespace hc {
 namespace {
@@ -28,14 +29,14 @@ template <typename T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-template <typename T, bool EXACT>
+template <typename T, bool EXACT, bool FUSED = false>
 __global__ void __launch_bounds__(THREADS)
 simt_gemm_kernel(const T* __restrict__ A, const T* __restrict__ B, T* __restrict__ C, const T* __restrict__ bias,
                  int64_t M, int64_t N, int64_t K,
                  int64_t a_rs, int64_t a_cs,   // A(m,k) = A[m*a_rs + k*a_cs]
                  int64_t b_rs, int64_t b_cs,   // B(k,n) = B[k*b_rs + n*b_cs]
                  int64_t ldc, int64_t strideA, int64_t strideB, int64_t strideC,
-                 int tiles_n) {
+                 int tiles_n, const FusedEpilogue fe) {
   __shared__ float As[BK][BM + 4];
   __shared__ float Bs[BK][BN + 4];
 
@@ -113,7 +114,21 @@ simt_gemm_kernel(const T* __restrict__ A, const T* __restrict__ B, T* __restrict
 #pragma unroll
     for (int j = 0; j < TN; j++) {
       int64_t gn = n0 + tx * TN + j;
-      if (gn < N) {
+      if (FUSED && gn < N) {
+        float x[1] = {acc[i][j]};
+        const int64_t off = gm * ldc + gn;
+        const float a = fe.aux ? to_float<T>(((const T*)fe.aux)[off]) : 0.0f;
+        if (fe.grad) {
+          const float pre[1] = {a};
+          act_scale<sizeof(T) == 2, 1>(fe.act, x, pre);
+        } else {
+          if (fe.bias) x[0] += to_float<T>(((const T*)fe.bias)[gn]);
+          if (fe.pre) ((T*)fe.pre)[off] = from_float<T>(x[0]);
+          act_apply<sizeof(T) == 2, 1>(fe.act, x);
+          if (fe.aux) x[0] += a;
+        }
+        C[off] = from_float<T>(x[0]);
+      } else if (gn < N) {
         T r = from_float<T>(acc[i][j]);
         // Linear's bias: a second operation on the rounded product (widen, add, narrow).
         if (bias) r = from_float<T>(__fadd_rn(to_float<T>(r), to_float<T>(bias[gn])));
@@ -129,7 +144,7 @@ cudaError_t launch_typed(const GemmProblem& p, bool exact, cudaStream_t stream, 
   const int64_t a_rs = p.a_mn_major ? 1 : p.lda, a_cs = p.a_mn_major ? p.lda : 1;
   const int64_t b_rs = p.b_mn_major ? p.ldb : 1, b_cs = p.b_mn_major ? 1 : p.ldb;
   if (rec) {
-    rec->kernel = exact ? HC_KERNEL_SIMT_EXACT : HC_KERNEL_SIMT;
+    rec->kernel = exact && !p.fused ? HC_KERNEL_SIMT_EXACT : HC_KERNEL_SIMT;
     rec->tile_m = BM; rec->tile_n = BN; rec->tile_k = BK; rec->stages = 1;
     rec->block = THREADS; rec->tiles = tiles_m * tiles_n * p.batch; rec->scratch_bytes = 0;
     rec->launches = 0;
@@ -141,14 +156,18 @@ cudaError_t launch_typed(const GemmProblem& p, bool exact, cudaStream_t stream, 
     const T* A = (const T*)p.A + b0 * p.strideA;
     const T* B = (const T*)p.B + b0 * p.strideB;
     T* C = (T*)p.C + b0 * p.strideC;
-    if (exact) {
+    if (p.fused) {
+      simt_gemm_kernel<T, false, true><<<grid, THREADS, 0, stream>>>(
+          A, B, C, nullptr, p.M, p.N, p.K, a_rs, a_cs, b_rs, b_cs, p.ldc, p.strideA, p.strideB, p.strideC,
+          (int)tiles_n, p.fe);
+    } else if (exact) {
       simt_gemm_kernel<T, true><<<grid, THREADS, 0, stream>>>(
           A, B, C, (const T*)p.bias, p.M, p.N, p.K, a_rs, a_cs, b_rs, b_cs, p.ldc, p.strideA, p.strideB, p.strideC,
-          (int)tiles_n);
+          (int)tiles_n, p.fe);
     } else {
       simt_gemm_kernel<T, false><<<grid, THREADS, 0, stream>>>(
           A, B, C, (const T*)p.bias, p.M, p.N, p.K, a_rs, a_cs, b_rs, b_cs, p.ldc, p.strideA, p.strideB, p.strideC,
-          (int)tiles_n);
+          (int)tiles_n, p.fe);
     }
     if (rec) { rec->launches++; rec->grid = (int)(tiles_m * tiles_n); }
     cudaError_t e = cudaGetLastError();

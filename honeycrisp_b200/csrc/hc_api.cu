@@ -5,6 +5,7 @@
 #include <mutex>
 #include <new>
 #include <string>
+#include <vector>
 
 #include <nvtx3/nvToolsExt.h>
 
@@ -13,6 +14,7 @@
 struct hc_ctx {
   int device = 0;
   cudaStream_t own_stream = nullptr;
+  cudaStream_t alloc_stream = nullptr;   // never captured: growth of the work area during a capture
   cudaStream_t stream = nullptr;
   std::mutex mu;
   unsigned int* status_word = nullptr;  // device memory
@@ -24,6 +26,10 @@ struct hc_ctx {
   // Work area of the float32 split operands; grown on demand, freed with the context.
   void* scratch = nullptr;
   size_t scratch_bytes = 0;
+  // A captured graph keeps the address of the work area it was captured with: once one has used it, an
+  // outgrown area is kept until the context goes instead of being freed.
+  bool scratch_in_graph = false;
+  std::vector<void*> retired_scratch;
   // Device staging buffers of the host-buffer entry point.
   void* stage[3] = {nullptr, nullptr, nullptr};
   size_t stage_bytes[3] = {0, 0, 0};
@@ -61,18 +67,7 @@ struct hc_event {
 
 namespace {
 
-struct DeviceGuard {
-  int prev = -1;
-  bool ok = true;
-  explicit DeviceGuard(int dev) {
-    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-    if (prev != dev) ok = (cudaSetDevice(dev) == cudaSuccess);
-  }
-  ~DeviceGuard() {
-    int cur = -1;
-    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
-  }
-};
+using hc::DeviceGuard;
 
 hc_status fail(hc_ctx* ctx, hc_status s, const std::string& msg) {
   if (ctx) ctx->last_error = msg;
@@ -128,6 +123,54 @@ hc_status ensure_buffer(hc_ctx* ctx, void** buf, size_t* have, size_t need, cuda
   }
   *buf = fresh;
   *have = bytes;
+  return HC_OK;
+}
+
+bool is_capturing(hc_ctx* ctx) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(ctx->stream, &st) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  return st != cudaStreamCaptureStatusNone;
+}
+
+// Grows the context's work area.  While the stream is being captured the memory must not become part
+// of the graph (an allocation node's address is the graph's alone, and the context goes on using it):
+// it is allocated on another stream, with this thread's capture checks relaxed for the moment.
+hc_status ensure_scratch(hc_ctx* ctx, size_t need) {
+  const bool capturing = is_capturing(ctx);
+  if (need <= ctx->scratch_bytes && ctx->scratch) {
+    if (capturing) ctx->scratch_in_graph = true;
+    return HC_OK;
+  }
+  if (!capturing && !ctx->scratch_in_graph)
+    return ensure_buffer(ctx, &ctx->scratch, &ctx->scratch_bytes, need, ctx->stream);
+  void* fresh = nullptr;
+  cudaError_t e;
+  try {
+    ctx->retired_scratch.reserve(ctx->retired_scratch.size() + 1);
+  } catch (...) {
+    return fail(ctx, HC_ERR_ALLOCATION_FAILED, "out of host memory");
+  }
+  if (capturing) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    e = ctx_malloc(ctx, &fresh, need, ctx->alloc_stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->alloc_stream);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+  } else {
+    e = ctx_malloc(ctx, &fresh, need, ctx->stream);
+  }
+  if (e != cudaSuccess) {
+    char msg[96];
+    snprintf(msg, sizeof msg, "allocation of %zu bytes failed", need);
+    return fail(ctx, HC_ERR_ALLOCATION_FAILED, msg);
+  }
+  if (ctx->scratch) ctx->retired_scratch.push_back(ctx->scratch);
+  ctx->scratch = fresh;
+  ctx->scratch_bytes = need;
+  if (capturing) ctx->scratch_in_graph = true;
   return HC_OK;
 }
 
@@ -190,12 +233,13 @@ cudaError_t launch_tensor(hc_ctx* ctx, const hc::GemmProblem& p, void* const* ex
   cudaError_t e = hc::launch_tc(p, ctx->stream, ctx->status_word, ctx->scratch, ctx->scratch_bytes, ctx->sm_count,
                                 &ctx->last, extra, n_extra, ctx->cache, &need, private_stream);
   if (e == cudaErrorInvalidValue && need > ctx->scratch_bytes) {
-    *st = ensure_buffer(ctx, &ctx->scratch, &ctx->scratch_bytes, need, ctx->stream);
+    *st = ensure_scratch(ctx, need);
     if (*st != HC_OK) return cudaErrorMemoryAllocation;
     hc::tc_cache_clear(ctx->cache);   // prepared launches point into the old work area
     e = hc::launch_tc(p, ctx->stream, ctx->status_word, ctx->scratch, ctx->scratch_bytes, ctx->sm_count, &ctx->last,
                       extra, n_extra, ctx->cache, &need, private_stream);
   }
+  if (e == cudaSuccess && ctx->last.scratch_bytes > 0 && !ctx->scratch_in_graph) ctx->scratch_in_graph = is_capturing(ctx);
   return e;
 }
 
@@ -224,7 +268,7 @@ hc_status run_problem(hc_ctx* ctx, hc_kernel kernel, const hc::GemmProblem& p, i
     return HC_OK;
   }
   const int64_t eb = p.dtype == HC_F16 ? 2 : 4;
-  if (p.K == 0) {
+  if (p.K == 0 && !p.fused) {
     // Empty contraction: every output is the empty sum, +0 (BackendCPU.swift:1293 starts at 0).
     for (int64_t m = 0; m < p.batch; m++) {
       HC_CUDA_TRY(ctx, cudaMemset2DAsync((char*)p.C + m * p.strideC * eb, p.ldc * eb, 0, p.N * eb, p.M, ctx->stream));
@@ -268,6 +312,17 @@ int64_t flop_count(int64_t count, int64_t rows, int64_t inner, int64_t cols) {
 
 // Accessors for the library's other translation units (hc_ctx is private to this file).
 namespace hc {
+hc_status ctx_run_problem(hc_ctx* ctx, const GemmProblem& p, int64_t flops) {
+  return run_problem(ctx, HC_KERNEL_AUTO, p, flops);
+}
+hc_status ctx_scratch(hc_ctx* ctx, size_t bytes, void** ptr) {
+  const void* before = ctx->scratch;
+  hc_status s = ensure_scratch(ctx, bytes);
+  if (s == HC_OK && ctx->scratch != before) tc_cache_clear(ctx->cache);   // prepared launches point into the old area
+  *ptr = s == HC_OK ? ctx->scratch : nullptr;
+  return s;
+}
+hc_status ctx_cuda_fail(hc_ctx* ctx, cudaError_t e, const char* what) { return cuda_fail(ctx, e, what); }
 std::mutex& ctx_mutex(hc_ctx* ctx) { return ctx->mu; }
 cudaStream_t ctx_stream(hc_ctx* ctx) { return ctx->stream; }
 unsigned int* ctx_status_word(hc_ctx* ctx) { return ctx->status_word; }
@@ -360,9 +415,11 @@ hc_status hc_init(int device, hc_ctx** out) {
   }
   ctx->sm_count = prop.multiProcessorCount;
   if (cudaStreamCreateWithFlags(&ctx->own_stream, cudaStreamNonBlocking) != cudaSuccess ||
+      cudaStreamCreateWithFlags(&ctx->alloc_stream, cudaStreamNonBlocking) != cudaSuccess ||
       cudaMalloc((void**)&ctx->status_word, sizeof(unsigned int)) != cudaSuccess ||
       cudaMemset(ctx->status_word, 0, sizeof(unsigned int)) != cudaSuccess) {
     if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
+    if (ctx->alloc_stream) cudaStreamDestroy(ctx->alloc_stream);
     if (ctx->status_word) cudaFree(ctx->status_word);
     delete ctx;
     cudaGetLastError();
@@ -398,6 +455,7 @@ void hc_destroy(hc_ctx* ctx) {
   if (ctx->trace_begin) cudaEventDestroy(ctx->trace_begin);
   if (ctx->trace_end) cudaEventDestroy(ctx->trace_end);
   if (ctx->scratch) cudaFreeAsync(ctx->scratch, ctx->own_stream);
+  for (void* old : ctx->retired_scratch) cudaFreeAsync(old, ctx->own_stream);
   for (int i = 0; i < 3; i++)
     if (ctx->stage[i]) cudaFreeAsync(ctx->stage[i], ctx->own_stream);
   for (auto& sl : ctx->slot) {
@@ -417,6 +475,7 @@ void hc_destroy(hc_ctx* ctx) {
     cudaStreamSynchronize(ctx->own_stream);
     cudaMemPoolDestroy(ctx->pool);
   }
+  cudaStreamDestroy(ctx->alloc_stream);
   cudaStreamDestroy(ctx->own_stream);
   cudaGetLastError();
   delete ctx;

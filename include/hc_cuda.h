@@ -225,6 +225,104 @@ hc_status hc_matmul_colblock(hc_ctx* ctx, hc_kernel kernel, hc_dtype dtype, cons
 hc_status hc_linear_forward(hc_ctx* ctx, hc_dtype dtype, const void* x, const void* weight,
                             const void* bias, int64_t rows, int64_t in_count, int64_t out_count,
                             void* out);
+/* Activations of the fused products.  GELU is z * Phi(z) with the normal distribution function;
+ * GELU_TANH its tanh form, z/2 * (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))); SILU z / (1 + exp(-z)). */
+typedef enum hc_activation {
+  HC_ACT_NONE = 0,
+  HC_ACT_RELU = 1,
+  HC_ACT_GELU = 2,
+  HC_ACT_GELU_TANH = 3,
+  HC_ACT_SILU = 4
+} hc_activation;
+
+/* What a product's epilogue does to each element before the result is rounded, once:
+ *   z = product + bias;  pre = z;  out = activation(z) + residual
+ * or, with grad_pre, the gradient form: out = product * activation'(grad_pre), which excludes bias,
+ * residual and pre.  Everything is computed in float32 on the unrounded product; any pointer may be
+ * NULL.  `bias` has `cols` elements, the others rows x cols, all of the product's dtype. */
+typedef struct hc_epilogue {
+  int activation;       /* hc_activation */
+  const void* bias;
+  const void* residual;
+  void* pre;            /* receives z: what the backward pass needs of the activation's input */
+  const void* grad_pre;
+} hc_epilogue;
+
+/* out[rows,cols] = epilogue(op(a) * op(b)); operands as in hc_matmul, without trans_out.  A feed-forward
+ * block is two of these forward (activation and pre; residual) and, backward, one with grad_pre
+ * between the plain weight-gradient products.  `out` may be the buffer of `residual` or of
+ * `grad_pre` (each element is read before it is written); no other overlap of `out` or `pre` with another
+ * tensor is allowed.  Differs from hc_linear_forward in rounding once, not after the product
+ * and again after the bias.
+ * Next to: Linear.callAsFunction (Trainable.swift:530-546) followed by an activation and an add. */
+hc_status hc_matmul_epilogue(hc_ctx* ctx, hc_dtype dtype, const void* a, int trans_a, const void* b,
+                             int trans_b, int64_t rows, int64_t inner, int64_t cols,
+                             const hc_epilogue* epilogue, void* out);
+/* dpre[rows,cols] = grad * activation'(pre), and, unless NULL, bias_grad[cols] (float32 whatever the
+ * dtype, as a layer's bias is) = the sum over rows of the unrounded dpre.  The sum's order depends on
+ * the shape alone.  `dpre` may be `grad`'s or `pre`'s buffer. */
+hc_status hc_activation_grad(hc_ctx* ctx, hc_dtype dtype, int activation, const void* grad,
+                             const void* pre, int64_t rows, int64_t cols, void* dpre,
+                             float* bias_grad);
+/* Layer normalisation over the last axis of x[rows,cols]:
+ *   out = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(variance + epsilon)
+ * `weight` and `bias` [cols] have `param_dtype` (a layer's are float32 whatever it computes in) and may be
+ * NULL (ones, zeros); `mean` and `rstd` [rows], float32, receive what the backward pass needs, unless NULL.
+ * Sums are float32, `out` is rounded once.  `out` may be `x`'s buffer.  `cols` is at least 1.
+ * Next to: Backend.normalize and LayerNorm of the reference (Backend.swift, Trainable.swift). */
+hc_status hc_layer_norm(hc_ctx* ctx, hc_dtype dtype, hc_dtype param_dtype, const void* x,
+                        const void* weight, const void* bias, int64_t rows, int64_t cols,
+                        float epsilon, void* out, float* mean, float* rstd);
+/* Its backward pass: `grad` is the gradient of `out`, `mean` and `rstd` what the forward pass stored.
+ *   dx = rstd * (g w - mean(g w) - h * mean(g w h)),  weight_grad = sum_rows g h,  bias_grad = sum_rows g
+ * with h = (x - mean) * rstd.  Any of the three results may be NULL; the parameters' gradients have
+ * `param_dtype`, are summed in float32 in an order that depends on shape and alignment alone, and are
+ * written, not accumulated.  `dx` may be `grad`'s or `x`'s buffer only when neither parameter gradient is asked for.
+ * Next to: Backend.normalizeGrad of the reference. */
+hc_status hc_layer_norm_grad(hc_ctx* ctx, hc_dtype dtype, hc_dtype param_dtype, const void* grad,
+                             const void* x, const void* weight, const float* mean,
+                             const float* rstd, int64_t rows, int64_t cols, void* dx,
+                             void* weight_grad, void* bias_grad);
+
+/* Products grouped by expert: rows offsets[g] to offsets[g+1] of `a` belong to group g.
+ *   out[r,cols] = a[r,inner] * op(b[g]),   b: group_count matrices [inner,cols], or [cols,inner] when trans_b
+ * `offsets` (group_count + 1, ascending, int64) lies on the device and is read there, when the call runs: the
+ * host waits for nothing, a captured graph follows new offsets, groups may be empty.  Rows of `out`
+ * before offsets[0] and from offsets[group_count] on are left as they are.  Offsets outside
+ * [0, total_rows] or running backwards are clamped to stay in range and ascending.  With trans_b this is
+ * also the gradient of the rows: d(a) = d(out) * b[g]^T.
+ * Next to: Backend.batchedMatmul (Backend.swift:661-669), whose matrices all have the same shape. */
+hc_status hc_grouped_matmul(hc_ctx* ctx, hc_dtype dtype, int64_t group_count,
+                            const int64_t* offsets, const void* a, const void* b, int trans_b,
+                            int64_t total_rows, int64_t inner, int64_t cols, void* out);
+/* The gradient of every group's matrix: out[g] = a_g^T * b_g [rows,cols], where a_g [n_g,rows] and
+ * b_g [n_g,cols] are the group's rows of a[total_rows,rows] and b[total_rows,cols]; zeros for a group
+ * without rows.  Offsets as above. */
+hc_status hc_grouped_matmul_weight_grad(hc_ctx* ctx, hc_dtype dtype, int64_t group_count,
+                                        const int64_t* offsets, const void* a, const void* b,
+                                        int64_t total_rows, int64_t rows, int64_t cols, void* out);
+
+/* One tensor of an AdamW step: `count` elements; the moments are float32, updated in place with `param`.
+ * `param_copy`, unless NULL, receives the new value in float16: the copy that a layer computing in
+ * float16 on float32 master weights reads next. */
+typedef struct hc_adamw_tensor {
+  void* param;
+  const void* grad;
+  float* moment1;
+  float* moment2;
+  void* param_copy;
+  int64_t count;
+  hc_dtype param_dtype, grad_dtype;
+} hc_adamw_tensor;
+/* One step over `tensor_count` tensors (a host array, read during the call), all in one launch for every
+ * few hundred of them:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr * weight_decay) - lr * (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + epsilon)
+ * in float32, `param` rounded once; `step` counts from 1.  The scalars are part of a captured launch: a
+ * replayed graph repeats the same step number.  No tensor may overlap another.
+ * Next to: Backend.adamW and Adam of the reference (Backend.swift, Optimizer.swift). */
+hc_status hc_adamw(hc_ctx* ctx, const hc_adamw_tensor* tensors, int64_t tensor_count, int64_t step,
+                   double lr, double beta1, double beta2, double epsilon, double weight_decay);
 /* out[cols] = sum over rows of x[rows,cols]: the bias gradient of a Linear layer.  One float
  * accumulator per column, rows in ascending order, narrowed once.
  * Replaces: Backend.reduce(.sum) over the leading axis as issued by reduceBroadcast
