@@ -150,11 +150,11 @@ size_t activation_grad_scratch(hc_dtype dtype, int64_t rows, int64_t cols);
 cudaError_t launch_activation_grad(hc_dtype dtype, int act, const void* grad, const void* pre, int64_t rows, int64_t cols,
                                    void* dpre, float* bias_grad, float* scratch, cudaStream_t stream);
 cudaError_t launch_layer_norm(hc_dtype dtype, hc_dtype param_dtype, const void* x, const void* w, const void* b, int64_t rows,
-                              int64_t cols, float epsilon, void* out, float* mean, float* rstd, cudaStream_t stream);
-size_t layer_norm_grad_scratch(hc_dtype dtype, int64_t rows, int64_t cols);
+                              int64_t cols, float epsilon, void* out, float* mean, float* rstd, int sm_count, cudaStream_t stream);
+size_t layer_norm_grad_scratch(hc_dtype dtype, int64_t rows, int64_t cols, int sm_count);
 cudaError_t launch_layer_norm_grad(hc_dtype dtype, hc_dtype param_dtype, const void* grad, const void* x, const void* w,
                                    const float* mean, const float* rstd, int64_t rows, int64_t cols, void* dx, void* dw, void* db,
-                                   float* scratch, int* launches, cudaStream_t stream);
+                                   float* scratch, int sm_count, int* launches, cudaStream_t stream);
 struct AdamWFactors { float lr, beta1, one_minus_beta1, beta2, one_minus_beta2, epsilon, decay, inv_c1, inv_c2; };
 cudaError_t launch_adamw(const hc_adamw_tensor* tensors, int64_t count, const AdamWFactors& f, int* launches, cudaStream_t stream);
 }  // namespace hc

@@ -121,7 +121,8 @@ hc_status hc_layer_norm(hc_ctx* ctx, hc_dtype dtype, hc_dtype param_dtype, const
   if ((overlap(so, sx) && !same(so, sx)) || overlap(so, sw) || overlap(so, sb) || overlap(so, sm) || overlap(so, sr) || overlap(sm, sx) ||
       overlap(sr, sx) || overlap(sm, sr) || overlap(sm, sw) || overlap(sm, sb) || overlap(sr, sw) || overlap(sr, sb))
     return invalid(ctx, "a result overlaps another tensor");
-  cudaError_t e = hc::launch_layer_norm(dtype, param_dtype, x, weight, bias, rows, cols, epsilon, out, mean, rstd, hc::ctx_stream(ctx));
+  cudaError_t e = hc::launch_layer_norm(dtype, param_dtype, x, weight, bias, rows, cols, epsilon, out, mean, rstd, hc::ctx_sm_count(ctx),
+                                        hc::ctx_stream(ctx));
   return launched(ctx, e, 1, "layer norm");
 }
 
@@ -153,12 +154,12 @@ hc_status hc_layer_norm_grad(hc_ctx* ctx, hc_dtype dtype, hc_dtype param_dtype, 
   if (!sums && (!dx || rows == 0)) return HC_OK;
   void* scratch = nullptr;
   if (sums) {
-    hc_status s = hc::ctx_scratch(ctx, hc::layer_norm_grad_scratch(dtype, rows, cols), &scratch);
+    hc_status s = hc::ctx_scratch(ctx, hc::layer_norm_grad_scratch(dtype, rows, cols, hc::ctx_sm_count(ctx)), &scratch);
     if (s != HC_OK) return s;
   }
   int launches = 0;
   cudaError_t e = hc::launch_layer_norm_grad(dtype, param_dtype, grad, x, weight, mean, rstd, rows, cols, dx, weight_grad, bias_grad,
-                                             (float*)scratch, &launches, hc::ctx_stream(ctx));
+                                             (float*)scratch, hc::ctx_sm_count(ctx), &launches, hc::ctx_stream(ctx));
   return launched(ctx, e, launches, "layer norm gradient");
 }
 
