@@ -15,10 +15,9 @@ namespace {
 constexpr int kLanes = 32, kWarps = 8;
 
 // kW: columns per lane; a 16-byte chunk, or 1 where rows are not 16-byte multiples.
-template <typename T, int kW, bool kSum>
+template <typename T, int kW, bool kSum, int kAct>
 __global__ void __launch_bounds__(kLanes * kWarps) activation_grad_kernel(const T* grad, const T* pre, T* dpre, float* partial,
-                                                                          int64_t rows, int64_t cols, int64_t rows_per_run,
-                                                                          int act) {
+                                                                          int64_t rows, int64_t cols, int64_t rows_per_run) {
   pdl_wait();
   if (kSum) pdl_release();   // the kernel behind sums the partial matrix and waits for this one
   const int lane = threadIdx.x % kLanes, warp = threadIdx.x / kLanes;
@@ -40,7 +39,7 @@ __global__ void __launch_bounds__(kLanes * kWarps) activation_grad_kernel(const 
         Pack16<T>::widen(gu, x);
         Pack16<T>::widen(zu, z);
       }
-      act_scale<sizeof(T) == 2, kW>(act, x, z);
+      act_scale_t<kAct, sizeof(T) == 2, kW>(x, z);
       if (kSum)
 #pragma unroll
         for (int e = 0; e < kW; e++) sum[e] += x[e];
@@ -112,14 +111,25 @@ cudaError_t launch_sum_runs(const float* partial, int64_t runs, int64_t cols, vo
 }
 
 namespace {
+template <typename T, int kAct>
+const void* kernel_of(bool vec, bool sum) {
+  constexpr int W = Pack16<T>::W;
+  return vec ? (sum ? (const void*)activation_grad_kernel<T, W, true, kAct> : (const void*)activation_grad_kernel<T, W, false, kAct>)
+             : (sum ? (const void*)activation_grad_kernel<T, 1, true, kAct> : (const void*)activation_grad_kernel<T, 1, false, kAct>);
+}
 template <typename T>
 cudaError_t launch_typed(const void* grad, const void* pre, int64_t rows, int64_t cols, void* dpre, float* bias_grad,
                          float* partial, bool vec, const RunSplit& s, int act, cudaStream_t stream) {
-  constexpr int W = Pack16<T>::W;
-  const void* fn = vec ? (bias_grad ? (const void*)activation_grad_kernel<T, W, true> : (const void*)activation_grad_kernel<T, W, false>)
-                       : (bias_grad ? (const void*)activation_grad_kernel<T, 1, true> : (const void*)activation_grad_kernel<T, 1, false>);
+  const void* fn = nullptr;
+  switch (act) {
+    case HC_ACT_RELU: fn = kernel_of<T, HC_ACT_RELU>(vec, bias_grad); break;
+    case HC_ACT_GELU: fn = kernel_of<T, HC_ACT_GELU>(vec, bias_grad); break;
+    case HC_ACT_GELU_TANH: fn = kernel_of<T, HC_ACT_GELU_TANH>(vec, bias_grad); break;
+    case HC_ACT_SILU: fn = kernel_of<T, HC_ACT_SILU>(vec, bias_grad); break;
+    default: fn = kernel_of<T, HC_ACT_NONE>(vec, bias_grad); break;
+  }
   int64_t per = s.rows_per_run;
-  void* args[] = {(void*)&grad, (void*)&pre, (void*)&dpre, (void*)&partial, (void*)&rows, (void*)&cols, (void*)&per, (void*)&act};
+  void* args[] = {(void*)&grad, (void*)&pre, (void*)&dpre, (void*)&partial, (void*)&rows, (void*)&cols, (void*)&per};
   cudaError_t e = launch_behind(fn, args, dim3((unsigned)s.strips, (unsigned)s.runs), dim3(kLanes * kWarps), 0, stream);
   if (e != cudaSuccess || !bias_grad) return e;
   return launch_sum_runs(partial, s.runs, cols, bias_grad, nullptr, false, stream);

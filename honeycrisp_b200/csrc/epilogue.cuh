@@ -8,6 +8,8 @@
 //
 // All of it happens in float32 on the unrounded product; each stored tensor is rounded once.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace hc {
@@ -17,17 +19,30 @@ namespace hc {
 //   GELU_TANH  S = sigma(2u), u = sqrt(2/pi) (z + 0.044715 z^3), which is (1 + tanh u) / 2 without its
 //              cancellation in the lower tail, where float16 still has 11 bits to fill
 //   GELU       S = Phi, the normal distribution function
-// so SILU and GELU_TANH share their code, sigma(k1 z + k3 z^3), and the slope is S + z S'.
+// and the slope is S + z S'.
 //
 // Phi(-y) = e^(-y^2/2) Q(y) for y >= 0 and Phi(y) = 1 - Phi(-y), where Q falls slowly from 1/2 and is fitted
 // by t R(t), t = 1/(1 + p y), R a polynomial, with least largest relative error over y <= 14 (Phi(-14) is
 // 8e-45, below float32's normals): degree 7, p = 0.3, 1.5e-7, for float32 results; degree 5, p = 0.31, 4.7e-6, for float16
 // ones, whose rounding is 4.9e-4.  In float32 the exponent's rounding dominates: 6e-7 of Phi at z = -3,
 // 1.3e-6 at -6.  kFast also takes the hardware's exponential and reciprocal (a few 2^-23).
+__device__ __forceinline__ float exp2_approx(float t) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+  return r;
+}
+// e^(c t), t's factor c folded into the base change where the exponential is the hardware's.
 template <bool kFast>
-__device__ __forceinline__ float exp_f(float t) { return kFast ? __expf(t) : expf(t); }
+__device__ __forceinline__ float exp_f(float c, float t) { return kFast ? exp2_approx(c * 1.4426950408889634f * t) : expf(c * t); }
 template <bool kFast>
-__device__ __forceinline__ float recip_f(float d) { return kFast ? __fdividef(1.0f, d) : 1.0f / d; }
+__device__ __forceinline__ float recip_f(float d) {
+  if (!kFast) return 1.0f / d;
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return r;
+}
+
+constexpr float kTanh1 = 1.5957691216057308f, kTanh3 = kTanh1 * 0.044715f;   // 2 sqrt(2/pi), and times 0.044715
 
 // Phi(z), and e^(-z^2/2) for the slope.
 template <bool kFast>
@@ -52,72 +67,70 @@ __device__ __forceinline__ float normal_cdf(float z, float& e) {
     r = fmaf(r, t, 0.12075395882129669f);
     r = fmaf(r, t, 0.11962930113077164f);
   }
-  e = exp_f<kFast>(-0.5f * y * y);
+  e = kFast ? exp2_approx(-0.72134752044448170f * y * y) : expf(-0.5f * y * y);
   const float tail = t * r * e;
   return z < 0.0f ? tail : 1.0f - tail;   // NaN: 1 - NaN
 }
 
-// The activation as the constants its code takes, so that one launch's choice costs a uniform branch:
-// kind 0 none, 1 ReLU, 2 sigma(k1 z + k3 z^3), 3 Phi.
-struct ActCode { int kind; float k1, k3; };
-__device__ __forceinline__ ActCode act_code(int act) {
-  ActCode c = {0, 1.0f, 0.0f};
-  if (act == HC_ACT_RELU) c.kind = 1;
-  if (act == HC_ACT_SILU) c.kind = 2;
-  if (act == HC_ACT_GELU_TANH) { c.kind = 2; c.k1 = 1.5957691216057308f; c.k3 = 1.5957691216057308f * 0.044715f; }
-  if (act == HC_ACT_GELU) c.kind = 3;
-  return c;
-}
-
-template <bool kFast, int W>
-__device__ __forceinline__ void act_apply(int act, float (&x)[W]) {
-  const ActCode c = act_code(act);
-  if (c.kind == 2) {
+template <int kAct, bool kFast, int W>
+__device__ __forceinline__ void act_apply_t(float (&x)[W]) {
 #pragma unroll
-    for (int e = 0; e < W; e++) {
-      const float z = x[e];
-      const float t = c.k3 != 0.0f ? z * fmaf(c.k3 * z, z, c.k1) : z;   // (0 z^3 is NaN at infinity)
-      x[e] = z * recip_f<kFast>(1.0f + exp_f<kFast>(-t));
+  for (int e = 0; e < W; e++) {
+    const float z = x[e];
+    if (kAct == HC_ACT_RELU) x[e] = z < 0.0f ? 0.0f : z;   // keeps NaN
+    if (kAct == HC_ACT_SILU) x[e] = z * recip_f<kFast>(1.0f + exp_f<kFast>(-1.0f, z));
+    if (kAct == HC_ACT_GELU_TANH) {
+      const float q = kFast ? exp2_approx(z * fmaf(-1.4426950408889634f * kTanh3 * z, z, -1.4426950408889634f * kTanh1))
+                            : expf(-z * fmaf(kTanh3 * z, z, kTanh1));
+      x[e] = z * recip_f<kFast>(1.0f + q);
     }
-  } else if (c.kind == 3) {
-#pragma unroll
-    for (int e = 0; e < W; e++) {
+    if (kAct == HC_ACT_GELU) {
       float g;
-      const float s = normal_cdf<kFast>(x[e], g);
-      x[e] *= s;
+      x[e] = z * normal_cdf<kFast>(z, g);
     }
-  } else if (c.kind == 1) {
-#pragma unroll
-    for (int e = 0; e < W; e++) x[e] = x[e] < 0.0f ? 0.0f : x[e];   // keeps NaN
   }
 }
 
 // x *= act'(pre).  sigma and 1 - sigma underflow together with the exponential's overflow, and inf * 0 must
 // not arise: beyond |z| = 16 (SILU 80) the slope is 0 or 1 to float32, so z is bounded there first.
-template <bool kFast, int W>
-__device__ __forceinline__ void act_scale(int act, float (&x)[W], const float (&pre)[W]) {
-  const ActCode c = act_code(act);
-  if (c.kind == 2) {
-    const float bound = c.k3 != 0.0f ? 16.0f : 80.0f;
+template <int kAct, bool kFast, int W>
+__device__ __forceinline__ void act_scale_t(float (&x)[W], const float (&pre)[W]) {
+  constexpr float kBound = kAct == HC_ACT_SILU ? 80.0f : 16.0f;
+  constexpr float k1 = kAct == HC_ACT_SILU ? 1.0f : kTanh1, k3 = kAct == HC_ACT_SILU ? 0.0f : kTanh3;
 #pragma unroll
-    for (int e = 0; e < W; e++) {
-      const float z = pre[e] != pre[e] ? pre[e] : fminf(fmaxf(pre[e], -bound), bound);
-      const float q = exp_f<kFast>(-fabsf(z) * fmaf(c.k3 * z, z, c.k1));   // in (0, 1]: both sigmas from it
+  for (int e = 0; e < W; e++) {
+    if (kAct == HC_ACT_RELU) x[e] = pre[e] <= 0.0f ? 0.0f : x[e];
+    const float z = pre[e] != pre[e] ? pre[e] : fminf(fmaxf(pre[e], -kBound), kBound);
+    if (kAct == HC_ACT_SILU || kAct == HC_ACT_GELU_TANH) {
+      const float q = exp_f<kFast>(-1.0f, fabsf(z) * fmaf(k3 * z, z, k1));   // in (0, 1]: both sigmas from it
       const float d = recip_f<kFast>(1.0f + q);
       const float s = z < 0.0f ? q * d : d;
-      x[e] *= fmaf(z * fmaf(3.0f * c.k3 * z, z, c.k1), q * d * d, s);
+      x[e] *= fmaf(z * fmaf(3.0f * k3 * z, z, k1), q * d * d, s);
     }
-  } else if (c.kind == 3) {
-#pragma unroll
-    for (int e = 0; e < W; e++) {
-      const float z = pre[e] != pre[e] ? pre[e] : fminf(fmaxf(pre[e], -16.0f), 16.0f);
+    if (kAct == HC_ACT_GELU) {
       float g;
       const float s = normal_cdf<kFast>(z, g);
       x[e] *= fmaf(z * 0.39894228040143268f, g, s);
     }
-  } else if (c.kind == 1) {
-#pragma unroll
-    for (int e = 0; e < W; e++) x[e] = pre[e] <= 0.0f ? 0.0f : x[e];
+  }
+}
+
+// A launch's epilogue as one number, so that a loop over a tile can be chosen once: the activation, plus
+// kGradCode in the gradient form.
+constexpr int kGradCode = 8;
+template <typename F>
+__device__ __forceinline__ void with_code(int act, int grad, F&& f) {
+  switch (act + (grad ? kGradCode : 0)) {
+    case HC_ACT_RELU: f(std::integral_constant<int, HC_ACT_RELU>()); break;
+    case HC_ACT_GELU: f(std::integral_constant<int, HC_ACT_GELU>()); break;
+    case HC_ACT_GELU_TANH: f(std::integral_constant<int, HC_ACT_GELU_TANH>()); break;
+    case HC_ACT_SILU: f(std::integral_constant<int, HC_ACT_SILU>()); break;
+    case kGradCode + HC_ACT_NONE: f(std::integral_constant<int, kGradCode + HC_ACT_NONE>()); break;
+    case kGradCode + HC_ACT_RELU: f(std::integral_constant<int, kGradCode + HC_ACT_RELU>()); break;
+    case kGradCode + HC_ACT_GELU: f(std::integral_constant<int, kGradCode + HC_ACT_GELU>()); break;
+    case kGradCode + HC_ACT_GELU_TANH: f(std::integral_constant<int, kGradCode + HC_ACT_GELU_TANH>()); break;
+    case kGradCode + HC_ACT_SILU: f(std::integral_constant<int, kGradCode + HC_ACT_SILU>()); break;
+    default: f(std::integral_constant<int, HC_ACT_NONE>()); break;
   }
 }
 
@@ -161,121 +174,38 @@ template <> struct Pack16<__half> {
   }
 };
 
-// The 16 bytes of elements [0, n) at p, the rest zero.
-template <typename T>
-__device__ __forceinline__ uint4 load16_partial(const T* p, int n) {
-  float x[Pack16<T>::W];
-#pragma unroll
-  for (int e = 0; e < Pack16<T>::W; e++) x[e] = e < n ? widen_f<T>(p[e]) : 0.0f;
-  return Pack16<T>::narrow(x);   // exact: the values came from T (a NaN's payload may change)
-}
-
-// One 16-byte chunk of a result row: x holds the float32 product of W columns, of which `n` exist
-// (n <= 0: none; nothing is read or written).  `off` is the chunk's element offset in every [M, N]
-// tensor, `col` its first column; `aux` its 16 bytes of the auxiliary tensor.
-template <typename T, int W>
-__device__ __forceinline__ void fused_chunk(const FusedEpilogue& f, int64_t off, int64_t col, int n, const uint4& aux,
-                                            float (&x)[W]) {
-  static_assert(W == Pack16<T>::W, "one 16-byte chunk");
-  constexpr bool kFast = sizeof(T) == 2;
-  if (f.grad) {
-    float pre[W];
-    Pack16<T>::widen(aux, pre);
-    act_scale<kFast, W>(f.act, x, pre);
-    return;
-  }
-  if (f.bias) {
-    const T* b = (const T*)f.bias + col;
-    float bv[W];
-    if (n >= W && ((uintptr_t)b & 15) == 0) {
-      Pack16<T>::widen(__ldg((const uint4*)b), bv);
-    } else {
-#pragma unroll
-      for (int e = 0; e < W; e++) bv[e] = e < n ? widen_f<T>(b[e]) : 0.0f;
-    }
-#pragma unroll
-    for (int e = 0; e < W; e++) x[e] += bv[e];
-  }
-  if (f.pre) {
-    T* dst = (T*)f.pre + off;
-    if (n >= W && f.vec) {
-      *(uint4*)dst = Pack16<T>::narrow(x);
-    } else {
-#pragma unroll
-      for (int e = 0; e < W; e++)
-        if (e < n) dst[e] = narrow_f<T>(x[e]);
-    }
-  }
-  act_apply<kFast, W>(f.act, x);
-  if (f.aux) {
-    float r[W];
-    Pack16<T>::widen(aux, r);
-#pragma unroll
-    for (int e = 0; e < W; e++) x[e] += r[e];
-  }
-}
-
-// kChunks consecutive 16-byte chunks of one row of the auxiliary tensor, of which `n` elements exist.
-template <typename T, int kChunks>
-__device__ __forceinline__ void load_aux(const FusedEpilogue& f, int64_t off, int64_t n, uint4 (&u)[kChunks]) {
-  constexpr int W = Pack16<T>::W;
-  if (f.aux && n > 0) {
-    const T* src = (const T*)f.aux + off;
-    if (f.vec && n >= kChunks * W) {
-#pragma unroll
-      for (int q = 0; q < kChunks; q++) u[q] = *(const uint4*)(src + q * W);   // not __ldg: it may be the result's own buffer
-    } else {
-#pragma unroll
-      for (int q = 0; q < kChunks; q++) {
-        const int64_t left = n - q * W;
-        u[q] = load16_partial<T>(src + q * W, left > W ? W : left < 0 ? 0 : (int)left);
-      }
-    }
+// The epilogue over W consecutive elements of a row, x the float32 product; `bias` and `aux` the W elements of those
+// tensors, widened (zero where a tensor is absent or the element lies outside).  z is what `pre` keeps.
+template <int kCode, bool kFast, int W>
+__device__ __forceinline__ void fused_values(float (&x)[W], const float (&bias)[W], const float (&aux)[W], float (&z)[W]) {
+  if constexpr (kCode >= kGradCode) {
+    act_scale_t<kCode - kGradCode, kFast, W>(x, aux);
   } else {
 #pragma unroll
-    for (int q = 0; q < kChunks; q++) u[q] = make_uint4(0, 0, 0, 0);
+    for (int e = 0; e < W; e++) z[e] = x[e] = x[e] + bias[e];
+    act_apply_t<kCode, kFast, W>(x);
+#pragma unroll
+    for (int e = 0; e < W; e++) x[e] += aux[e];
   }
 }
 
-// The same over 32 consecutive columns of a row, for the paths that store from registers.
-template <typename T>
-__device__ __forceinline__ void fused_row32(const FusedEpilogue& f, int64_t off, int64_t col, int64_t n, float (&v)[32]) {
-  constexpr int W = Pack16<T>::W;
-  uint4 aux[32 / W];
-  load_aux<T, 32 / W>(f, off, n, aux);
-#pragma unroll
-  for (int q = 0; q < 32 / W; q++) {
-    float x[W];
-#pragma unroll
-    for (int e = 0; e < W; e++) x[e] = v[q * W + e];
-    const int64_t left = n - q * W;
-    fused_chunk<T, W>(f, off + q * W, col + q * W, left > W ? W : left < 0 ? 0 : (int)left, aux[q], x);
-#pragma unroll
-    for (int e = 0; e < W; e++) v[q * W + e] = x[e];
-  }
-}
-
-// The same over four consecutive columns, element by element: for the kernel that sums the parts of a
-// cut contraction, whose time goes into reading the parts.
-template <typename T>
-__device__ __forceinline__ void fused_four(const FusedEpilogue& f, int64_t off, int64_t col, int n, float (&x)[4]) {
+// The same over four consecutive columns in memory, element by element: for the CUDA-core kernel and for the kernel that sums
+// the parts of a cut contraction, whose time goes elsewhere.  `off` is the element offset in every [M, N] tensor.
+template <typename T, int W>
+__device__ __forceinline__ void fused_direct(const FusedEpilogue& f, int64_t off, int64_t col, int n, float (&x)[W]) {
   constexpr bool kFast = sizeof(T) == 2;
-  float a[4];
+  float a[W], b[W], z[W];
 #pragma unroll
-  for (int e = 0; e < 4; e++) a[e] = (f.aux && e < n) ? widen_f<T>(((const T*)f.aux)[off + e]) : 0.0f;
-  if (f.grad) {
-    act_scale<kFast, 4>(f.act, x, a);
-    return;
+  for (int e = 0; e < W; e++) {
+    a[e] = (f.aux && e < n) ? widen_f<T>(((const T*)f.aux)[off + e]) : 0.0f;
+    b[e] = (f.bias && e < n) ? widen_f<T>(((const T*)f.bias)[col + e]) : 0.0f;
+    z[e] = 0.0f;
   }
+  with_code(f.act, f.grad, [&](auto code) { fused_values<decltype(code)::value, kFast, W>(x, b, a, z); });
+  if (f.pre)
 #pragma unroll
-  for (int e = 0; e < 4; e++) {
-    if (f.bias && e < n) x[e] += widen_f<T>(((const T*)f.bias)[col + e]);
-    if (f.pre && e < n) ((T*)f.pre)[off + e] = narrow_f<T>(x[e]);
-  }
-  act_apply<kFast, 4>(f.act, x);
-  if (f.aux)
-#pragma unroll
-    for (int e = 0; e < 4; e++) x[e] += a[e];
+    for (int e = 0; e < W; e++)
+      if (e < n) ((T*)f.pre)[off + e] = narrow_f<T>(z[e]);
 }
 
 }  // namespace hc

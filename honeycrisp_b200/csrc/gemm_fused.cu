@@ -4,7 +4,7 @@
 
 namespace hc {
 
-TcLaunchFn fused_kernel(bool f32, int shape, int kslabs, int short_k) {
+TcLaunchFn fused_kernel(bool f32, int shape) {
   if (f32) {
     switch (shape) {
       case SHAPE_PAIR_128: return TcConfig<4, 128, 3, 4, true, 2, 1, 1, false, kFused>::launch;
@@ -16,14 +16,12 @@ TcLaunchFn fused_kernel(bool f32, int shape, int kslabs, int short_k) {
     }
   }
   switch (shape) {
-    case SHAPE_WIDE: return TcConfig<2, 256, 4, 8, false, 2, 2, 1, false, kFused>::launch;
-    case SHAPE_PAIR_128: return TcConfig<2, 128, 4, 4, false, 2, 1, 2, false, kFused>::launch;
+    case SHAPE_PAIR_128: return TcConfig<2, 128, 3, 4, false, 2, 1, 2, false, kFused>::launch;
     case SHAPE_PAIR_64: return TcConfig<2, 64, 4, 4, false, 2, 1, 2, false, kFused>::launch;
     case SHAPE_PAIR:
-      if (kslabs <= short_k) return TcConfig<2, 256, 4, 8, false, 2, 1, 1, false, kFused>::launch;
-      return TcConfig<2, 256, 6, 4, false, 2, 1, 1, false, kFused>::launch;
-    case SHAPE_C1_256: return TcConfig<2, 256, 4, 4, false, 1, 1, 1, false, kFused>::launch;
-    case SHAPE_C1_128: return TcConfig<2, 128, 3, 4, false, 1, 1, 2, false, kFused>::launch;
+      return TcConfig<2, 256, 4, 8, false, 2, 1, 1, false, kFused>::launch;
+    case SHAPE_C1_256: return TcConfig<2, 256, 3, 4, false, 1, 1, 1, false, kFused>::launch;
+    case SHAPE_C1_128: return TcConfig<2, 128, 5, 4, false, 1, 1, 1, false, kFused>::launch;
     default: return nullptr;
   }
 }

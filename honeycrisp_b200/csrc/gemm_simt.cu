@@ -117,16 +117,7 @@ simt_gemm_kernel(const T* __restrict__ A, const T* __restrict__ B, T* __restrict
       if (FUSED && gn < N) {
         float x[1] = {acc[i][j]};
         const int64_t off = gm * ldc + gn;
-        const float a = fe.aux ? to_float<T>(((const T*)fe.aux)[off]) : 0.0f;
-        if (fe.grad) {
-          const float pre[1] = {a};
-          act_scale<sizeof(T) == 2, 1>(fe.act, x, pre);
-        } else {
-          if (fe.bias) x[0] += to_float<T>(((const T*)fe.bias)[gn]);
-          if (fe.pre) ((T*)fe.pre)[off] = from_float<T>(x[0]);
-          act_apply<sizeof(T) == 2, 1>(fe.act, x);
-          if (fe.aux) x[0] += a;
-        }
+        fused_direct<T, 1>(fe, off, gn, 1, x);
         C[off] = from_float<T>(x[0]);
       } else if (gn < N) {
         T r = from_float<T>(acc[i][j]);

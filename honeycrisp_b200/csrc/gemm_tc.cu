@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(256) splitk_reduce_kernel(const ReduceJob j) {
     if (kFusedSum) {
       typedef typename std::conditional<kHalf, __half, float>::type T;
       const int64_t off = mat * j.strideC + row * j.ldc + n;
-      fused_four<T>(j.fe, off, n, valid, x);
+      fused_direct<T, 4>(j.fe, off, n, valid, x);
       T* dst = (T*)j.C + off;
       T r[4];
 #pragma unroll
@@ -193,7 +193,8 @@ TcPlan plan_tc(const GemmProblem& p, int sm_count, bool may_split, const Tunable
   Cand cands[SHAPE_COUNT - 1];
   int n_cands = 0;
   if (!f32) {
-    const bool wide_ok = pairs_ok && N >= 1024 && kslabs >= tun.wide_min_kb;
+    // A fused epilogue takes longer than the half-by-half drain of the 512-wide tile hides.
+    const bool wide_ok = pairs_ok && N >= 1024 && kslabs >= tun.wide_min_kb && !p.fused;
     cands[n_cands++] = {SHAPE_WIDE, wide_ok, 256, 512, pair_slots, 1, 1140.0, drain, false};
     cands[n_cands++] = {SHAPE_PAIR, pairs_ok && N > 128, 256, 256, pair_slots, 1, 600.0, 0.0, true};
     cands[n_cands++] = {SHAPE_C1_256, N > 128, 128, 256, sm_count, 1, 680.0, 0.0, false};
@@ -484,7 +485,9 @@ cudaError_t prepare_tc(const GemmProblem& p, unsigned int* status_word, void* sc
   // memory load, conversion, proxy fence and TMA store, and more chains in flight hide more of
   // it - measured +8 % at K = 128, nothing at K = 256, -3 % at K = 512) and fewer operand stages.
   const bool short_k = kslabs <= tun.short_k;
-  const int slabs = plan.slabs;   // pipeline slots of the small float16 shapes hold two k slabs
+  // Pipeline slots of the small float16 shapes hold two k slabs; the fused 128x128 tile, whose staging ring leaves room for
+  // only two such slots, has five of one.
+  const int slabs = (p.fused && plan.splits == 1 && !f32 && shape == SHAPE_C1_128) ? 1 : plan.slabs;
   tp.num_k_blocks = (kslabs + slabs - 1) / slabs;
   const bool cut = plan.splits > 1;
   tp.splits = plan.splits;
@@ -516,6 +519,11 @@ cudaError_t prepare_tc(const GemmProblem& p, unsigned int* status_word, void* sc
   tp.fe = p.fe;
   // 16-byte accesses to the tensors laid out like the result
   tp.fe.vec = ((((uintptr_t)p.fe.aux | (uintptr_t)p.fe.pre) & 15) == 0 && (p.ldc * eb) % 16 == 0) ? 1 : 0;
+  if (p.fused && !cut && tp.fe.vec) {
+    // maps 1 and 2 of the results' array: the kept pre-activation and the auxiliary tensor
+    if (p.fe.pre && !make_output_map(&pp.outs.m[1], p.fe.pre, eb, p.N, p.M, p.ldc, p.strideC, p.batch)) return cudaErrorNotSupported;
+    if (p.fe.aux && !make_output_map(&pp.outs.m[2], const_cast<void*>(p.fe.aux), eb, p.N, p.M, p.ldc, p.strideC, p.batch)) return cudaErrorNotSupported;
+  }
   if (cut) {
     const size_t off = (ops_bytes + 255) & ~(size_t)255;
     out_base = (char*)scratch + off;
@@ -564,7 +572,7 @@ cudaError_t prepare_tc(const GemmProblem& p, unsigned int* status_word, void* sc
   TcLaunchFn fn = nullptr;
   if (p.fused && !cut) {
     if (f32 && !windowed) return cudaErrorInvalidValue;   // the fused epilogue is not built for the no-window debug mode
-    fn = fused_kernel(f32, shape, kslabs, tun.short_k);
+    fn = fused_kernel(f32, shape);
     if (!fn) return cudaErrorInvalidValue;
   } else if (!f32 && cut) {
     if (shape == SHAPE_PAIR_128) fn = TcConfig<2, 128, 4, 4, false, 2, 1, 2, true>::launch;

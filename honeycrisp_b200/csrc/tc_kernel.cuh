@@ -123,9 +123,8 @@ typedef cudaError_t (*TcLaunchFn)(const CUtensorMap maps[4], const OutMaps& outs
 
 enum Shape { SHAPE_AUTO = 0, SHAPE_WIDE, SHAPE_PAIR, SHAPE_C1_256, SHAPE_C1_128, SHAPE_PAIR_128, SHAPE_PAIR_64,
              SHAPE_COUNT };
-// The kernel with the fused epilogue for a tile shape (csrc/gemm_fused.cu); `slabs` is the number of
-// k slabs of the contraction.
-TcLaunchFn fused_kernel(bool f32, int shape, int kslabs, int short_k);
+// The kernel with the fused epilogue for a tile shape (csrc/gemm_fused.cu); null where it is not built.
+TcLaunchFn fused_kernel(bool f32, int shape);
 
 namespace {
 
@@ -385,6 +384,16 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -493,24 +502,52 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(addr) : "memory");
   return u;
 }
-// The fused epilogue over one lane's row of 32 float32 columns in its swizzled staging buffer: back into
-// the buffer for a TMA store, or to memory where TMA cannot describe the result.
-__device__ __noinline__ void fused_staged32(const TcParams& p, uint32_t row_addr, uint32_t sw, int64_t off, int64_t col,
-                                            int64_t left, const uint4 (&aux)[8]) {
-#pragma unroll 1
-  for (int q = 0; q < 8; q++) {
-    const uint32_t at = row_addr + (((uint32_t)q ^ sw) << 4);
-    float x[4];
-    Pack16<float>::widen(ld_shared_v4(at), x);
-    const int64_t n = left - q * 4;
-    fused_chunk<float, 4>(p.fe, off + q * 4, col + q * 4, (int)(n > 4 ? 4 : n < 0 ? 0 : n), aux[q], x);
-    if (p.tma_store) {
-      const uint4 u = Pack16<float>::narrow(x);
-      st_shared_v4(at, u.x, u.y, u.z, u.w);
-    } else {
+__device__ __forceinline__ uint32_t ld_shared_b32(uint32_t addr) {
+  uint32_t u;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(u) : "r"(addr) : "memory");
+  return u;
+}
+__device__ __forceinline__ void st_shared_b32(uint32_t addr, uint32_t u) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(u) : "memory");
+}
+// A staging block (32 rows x 128 bytes, 16-byte units swizzled by the row) and memory, by the whole warp, a row at a time:
+// for tensors that cannot be described to TMA.  `base` points at the block's first element, `rows` x `cols` of it exist.
+template <typename T>
+__device__ __noinline__ void block_to_memory(uint32_t buf, T* base, int64_t ld, int rows, int cols) {
+  const int lane = threadIdx.x & 31;
+  constexpr int V = 4 / (int)sizeof(T);
+#pragma unroll 4
+  for (int r = 0; r < rows; r++) {
+    const uint32_t u = ld_shared_b32(buf + r * 128 + ((uint32_t)((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+    const T* v = (const T*)&u;
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (e < n) ((float*)p.C)[off + q * 4 + e] = x[e];
+    for (int e = 0; e < V; e++)
+      if (lane * V + e < cols) base[r * ld + lane * V + e] = v[e];
+  }
+}
+// Into a staging block; the loads of many rows are under way before the first is needed.
+template <typename T>
+__device__ __noinline__ void block_from_memory(uint32_t buf, const T* base, int64_t ld, int rows, int cols) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (sizeof(T) == 4) {
+    if (lane < cols)
+      for (int r = 0; r < rows; r++)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(buf + r * 128 + ((uint32_t)((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4),
+                     "l"(base + r * ld + lane) : "memory");
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else {
+    for (int r0 = 0; r0 < rows; r0 += 16) {
+      uint32_t u[16];
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const T* src = base + (r0 + i) * ld + lane * 2;
+        const T lo = r0 + i < rows && lane * 2 < cols ? src[0] : (T)0.0f, hi = r0 + i < rows && lane * 2 + 1 < cols ? src[1] : (T)0.0f;
+        const __half2 h = __halves2half2(lo, hi);
+        u[i] = *(const uint32_t*)&h;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        st_shared_b32(buf + (r0 + i) * 128 + ((uint32_t)((lane >> 2) ^ (i & 7)) << 4) + (lane & 3) * 4, u[i]);
     }
   }
 }
@@ -545,6 +582,9 @@ __device__ __forceinline__ TileCoord decode_tile(int64_t tile, const TcParams& p
 __host__ __device__ constexpr int staging_bufs(int out_bytes, int bn, int epi_warps, bool windowed, int nsplit) {
   return (windowed || (epi_warps == 8 && nsplit == 2) || (bn * nsplit / (epi_warps / 4)) < 2 * (128 / out_bytes)) ? 1 : 2;
 }
+
+// The fused float16 epilogue stages every tensor of the result's shape: three buffers a warp in a ring.
+__host__ __device__ constexpr bool staging_ring(int mode, bool windowed) { return mode == 1 && !windowed; }
 
 // With the contraction cut into parts, tiles are numbered over batch x parts "matrices": the
 // operands of matrix v / parts, k slots [kb0, kb0 + count), the result into partial matrix v.
@@ -597,6 +637,61 @@ __device__ __forceinline__ KRange k_range(int64_t vmat, const TcParams& p) {
   return r;
 }
 
+// The fused epilogue over a float32 staging block: every lane works on its own row's chunks, in place; where z is kept, the
+// block leaves once before the activation and once behind it.
+__device__ __noinline__ void fused_block(const TcParams& p, const OutMaps& mapC, uint32_t buf, const uint4 (&aux)[8], int row, int col,
+                                         int rows_here, int cols_here, bool store_leader) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t sw = (uint32_t)(lane & 7);
+  const bool tma = p.tma_store && p.fe.vec;
+  auto leave = [&](const CUtensorMap* map, void* base) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (tma) {
+      if (store_leader) {
+        tma_store_3d(map, buf, col, row, 0);
+        bulk_commit();
+      }
+    } else {
+      block_to_memory<float>(buf, (float*)base + (int64_t)row * p.ldc + col, p.ldc, rows_here, cols_here);
+    }
+  };
+  if (!p.fe.grad && p.fe.bias) {
+#pragma unroll 1
+    for (int q = 0; q < 8; q++) {
+      const uint32_t at = buf + (uint32_t)lane * 128u + (((uint32_t)q ^ sw) << 4);
+      float x[4];
+      Pack16<float>::widen(ld_shared_v4(at), x);
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (q * 4 + e < cols_here) x[e] += __ldg((const float*)p.fe.bias + col + q * 4 + e);
+      const uint4 u = Pack16<float>::narrow(x);
+      st_shared_v4(at, u.x, u.y, u.z, u.w);
+    }
+  }
+  if (p.fe.pre) {
+    leave(&mapC.m[1], p.fe.pre);
+    if (tma && store_leader) bulk_wait_read<0>();
+    __syncwarp();
+  }
+  with_code(p.fe.act, p.fe.grad, [&](auto code) {
+    constexpr int kCode = decltype(code)::value;
+#pragma unroll 1
+    for (int q = 0; q < 8; q++) {
+      const uint32_t at = buf + (uint32_t)lane * 128u + (((uint32_t)q ^ sw) << 4);
+      const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      float x[4], a[4] = {0.0f, 0.0f, 0.0f, 0.0f}, z[4];
+      Pack16<float>::widen(ld_shared_v4(at), x);
+      if (p.fe.aux) Pack16<float>::widen(aux[q], a);
+      fused_values<kCode, false, 4>(x, none, a, z);
+      const uint4 u = Pack16<float>::narrow(x);
+      st_shared_v4(at, u.x, u.y, u.z, u.w);
+    }
+  });
+  leave(&mapC.m[0], p.C);
+  __syncwarp();
+}
+
 // kElemBytes: 2 (float16 operands) or 4 (float32 operands consumed as TF32).
 // kBN       : columns of one tcgen05.mma (and of one accumulator buffer).
 // kNSplit   : 1, or 2 for tiles two MMAs wide (512 columns) whose halves take the two accumulator
@@ -642,7 +737,8 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
   constexpr uint32_t A_BYTES = BM * 128, B_PART_BYTES = BN_LOCAL * 128, B_BYTES = kNSplit * B_PART_BYTES,
                      SLAB_BYTES = PARTS * (A_BYTES + B_BYTES), STAGE_BYTES = kSlabs * SLAB_BYTES;
   static_assert(kSlabs == 1 || !kWindowed, "accumulation windows count single slabs");
-  constexpr int STG_BUFS = staging_bufs(kOutHalf ? 2 : 4, kBN, kEpiWarps, kWindowed, kNSplit);
+  constexpr bool kRing = staging_ring(kMode, kWindowed);
+  constexpr int STG_BUFS = kRing ? 3 : staging_bufs(kOutHalf ? 2 : 4, kBN, kEpiWarps, kWindowed, kNSplit);
   constexpr uint32_t STG_BYTES_PER_WARP = STG_BUFS * 4096u;
   constexpr int TMEM_COLS = (2 * kBN <= 32) ? 32 : 2 * kBN;
   constexpr int COL_SPLIT = kEpiWarps / 4;   // epilogue warps sharing one lane quarter
@@ -653,7 +749,7 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
   static_assert(kCta == 1 || kCta == 2, "one CTA or a pair");
 
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * kStages + 4];
+  __shared__ __align__(8) uint64_t bars[2 * kStages + 4 + (kRing ? 3 * kEpiWarps : 0)];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
 
@@ -675,6 +771,7 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
       mbar_init(bar_tfull + 8 * s, 1);
       mbar_init(bar_tempty + 8 * s, 32 * kEpiWarps * kCta);
     }
+    for (int i = 0; kRing && i < 3 * kEpiWarps; i++) mbar_init(bar_tempty + 16 + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -1029,6 +1126,24 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
     pdl_wait();
     if (warp == 2 && store_leader) pdl_release();   // one thread per CTA is enough
     const int64_t total_tiles = kMode == kGrouped ? p.groups.first_tile[p.groups.count] : p.total_tiles;
+    // Ring of staging buffers (kRing): the tensors of the result's shape go by TMA where all of them can be described to it.
+    const bool ring_tma = kRing && p.tma_store && p.fe.vec;
+    const bool aux_tma = ring_tma && p.fe.aux;
+    const uint32_t bar_aux = bar_tempty + 16 + 24 * (uint32_t)ew;
+    uint32_t ring_use = 0, ring_pass = 0;
+    const int aux_ahead = p.fe.pre ? 1 : 2;   // passes; a kept pre-activation takes every other buffer
+    auto fetch_aux = [&](uint32_t use, int64_t tile, int pass) {   // one lane; passes beyond the tile's are the next tiles'
+      constexpr int kPasses = kRing ? kBN / COL_SPLIT / 64 : 1;
+      while (pass >= kPasses) { pass -= kPasses; tile += tile_step; }
+      if (tile >= total_tiles) return;
+      const TileCoord at = decode_tile(tile, p);
+      const uint32_t buf = use % 3;
+      mbar_expect_tx(bar_aux + 8 * buf, 4096);
+      tma_load_3d<1>(stg_base + buf * 4096u, &mapC.m[2], bar_aux + 8 * buf, at.tn * TILE_N + col_part * (kBN / COL_SPLIT) + 64 * pass,
+                     at.tm * (BM * kCta) + (int)rank * BM + quarter * 32, 0);
+    };
+    if (aux_tma && store_leader)
+      for (int i = 0; i < aux_ahead; i++) fetch_aux(p.fe.pre ? 1 : i, tile_first, i);
     for (int64_t tile = tile_first; ok && tile < total_tiles; tile += tile_step) {
       if (kMode != kGrouped && tile != tile_first) t = decode_tile(tile, p);
       int64_t row0 = 0, row_end = p.M;   // result rows this tile may write
@@ -1068,12 +1183,6 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
         for (int h = 0; h < kNSplit && ok; h++) {
         const uint32_t slot = (kNSplit == 2) ? (uint32_t)h : win % ACC_SLOTS;
         const uint32_t par = (kNSplit == 2) ? (win & 1) : ((win / ACC_SLOTS) & 1);
-        // Fused epilogue: the auxiliary tensor's part of 32 columns is read 32 columns ahead, the first
-        // ones under the wait for the accumulator.
-        constexpr int CHUNKS32 = kOutHalf ? 4 : 8;   // 16-byte chunks of 32 results
-        uint4 aux[kMode == kFused ? CHUNKS32 : 1];
-        const int64_t fcol0 = (int64_t)t.tn * TILE_N + h * kBN + col_part * COLS_PER_PART;
-        if (kMode == kFused && p.tma_store) load_aux<OutT>(p.fe, row_off + fcol0, gm < p.M ? p.N - fcol0 : 0, aux);
         const bool got = mbar_wait_warp(bar_tfull + 8 * slot, par, abortp, lane);
         if (!got) {
           if (lane == 0) { atomicOr(p.status, kDevTimeoutEpilogue); abort_flag = 1; }
@@ -1084,52 +1193,113 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
         const int part0 = col_part * COLS_PER_PART;
         const uint32_t tbase = tmem_base + lane_base + slot * kBN + part0;
         const int64_t n0h = (int64_t)t.tn * TILE_N + h * kBN + part0;
-        if (kMode == kFused && p.tma_store) {
-          // Columns in units of 32, one tensor-memory load each, so that the epilogue's arithmetic
-          // exists once in the code; the staging buffers (64 float16 columns or 32 float32 ones)
-          // alternate as they fill.
-          constexpr int W = Pack16<OutT>::W;
-          constexpr int COLS_PER_BUF = 8 * W;
-          const int m_warp = t.tm * (BM * kCta) + (int)rank * BM + quarter * 32;
+        if constexpr (kRing) {
+          // 64 columns a pass.  Every block of 32 rows x 128 bytes that leaves (the result, the kept pre-activation) or
+          // enters (the auxiliary tensor, whose block the result then overwrites) takes the next of three buffers; a
+          // block's own bulk group tells when its buffer has been read.  Auxiliary blocks are fetched ahead.
+          // The loops are rolled and exist once for every kind of epilogue: unrolled over a tile with the choice inside,
+          // their code outgrew the instruction cache (8192 x 512 x 8192, no extras: 109 us against RINGNONE).
+          constexpr int W = 8;
+          static_assert(!kRing || COLS_PER_PART % 64 == 0, "whole passes");
           const uint32_t sw = (uint32_t)(lane & 7);
+          const int m_warp = (int)(gm - lane);
+          const int rows_here = (int)min((int64_t)32, p.M - m_warp);   // may be negative
+          with_code(p.fe.act, p.fe.grad, [&](auto code) {
+            constexpr int kCode = decltype(code)::value;
+            uint32_t n[16];   // the next 16 columns, on their way out of tensor memory
+            tmem_ld_x16(tbase, n);
 #pragma unroll 1
-          for (int c = 0; c < COLS_PER_PART; c += 32) {
-            const uint32_t buf = stg_base + (uint32_t)((c / COLS_PER_BUF) % STG_BUFS) * 4096u;
-            const uint32_t chunk0 = (uint32_t)(c % COLS_PER_BUF) / W;   // first 16-byte chunk of the row
-            uint32_t r[32];
-            tmem_ld_x32(tbase + c, r);
-            if (chunk0 == 0) {   // the store that last read this buffer has had the other buffer's turn
-              if (store_leader) bulk_wait_read<STG_BUFS - 1>();
+            for (int c = 0; c < COLS_PER_PART; c += 64) {
+              const int64_t col0 = n0h + c;
+              const int cols_here = (int)min((int64_t)64, p.N - col0);
+              uint32_t pre_buf = 0;
+              if (kCode < kGradCode && p.fe.pre) {
+                if (store_leader) bulk_wait_read<1>();   // two buffers at once: of the groups before, all but the last
+                pre_buf = stg_base + (ring_use % 3) * 4096u;
+                ring_use++;
+              }
+              const uint32_t out_buf = stg_base + (ring_use % 3) * 4096u;
+              if (aux_tma) {
+                if (!mbar_wait_warp(bar_aux + 8 * (ring_use % 3), (ring_pass / 3) & 1, abortp, lane)) { ok = false; break; }
+              } else if (!(kCode < kGradCode && p.fe.pre)) {
+                if (store_leader) bulk_wait_read<2>();
+              }
               __syncwarp();
-            }
-            tmem_ld_wait();
+              if (p.fe.aux && !aux_tma) {
+                if (rows_here > 0 && cols_here > 0)
+                  block_from_memory<__half>(out_buf, (const __half*)p.fe.aux + (int64_t)m_warp * p.ldc + col0, p.ldc, rows_here, cols_here);
+                __syncwarp();
+              }
+#pragma unroll 1
+              for (int k = 0; k < 64; k += 16) {
+                tmem_ld_wait();
+                uint32_t r[16];
 #pragma unroll
-            for (int q = 0; q < CHUNKS32; q++) {
-              float x[W];
+                for (int i = 0; i < 16; i++) r[i] = n[i];
+                if (c + k + 16 < COLS_PER_PART) tmem_ld_x16(tbase + c + k + 16, n);
 #pragma unroll
-              for (int e = 0; e < W; e++) x[e] = __uint_as_float(r[q * W + e]);
-              const int64_t col = n0h + c + q * W;
-              fused_chunk<OutT, W>(p.fe, row_off + col, col, gm < p.M ? (int)(p.N - col) : 0, aux[kMode == kFused ? q : 0], x);
-              const uint4 u = Pack16<OutT>::narrow(x);
-              st_shared_v4(buf + (uint32_t)lane * 128u + (((chunk0 + q) ^ sw) << 4), u.x, u.y, u.z, u.w);
-            }
-            if (c + 32 < COLS_PER_PART) load_aux<OutT>(p.fe, row_off + n0h + c + 32, gm < p.M ? p.N - n0h - c - 32 : 0, aux);
-            if (chunk0 + CHUNKS32 == 8) {
+                for (int q = 0; q < 2; q++) {
+                  float x[W], bias[W], aux[W], z[W];
+                  const uint32_t at = (uint32_t)lane * 128u + (((uint32_t)(k / W + q) ^ sw) << 4);
+#pragma unroll
+                  for (int e = 0; e < W; e++) { x[e] = __uint_as_float(r[q * W + e]); bias[e] = aux[e] = 0.0f; }
+                  if (kCode < kGradCode && p.fe.bias) {
+                    const __half* b = (const __half*)p.fe.bias + col0 + k + q * W;
+                    if (cols_here >= k + (q + 1) * W && ((uintptr_t)b & 15) == 0) {
+                      Pack16<__half>::widen(__ldg((const uint4*)b), bias);
+                    } else {
+#pragma unroll
+                      for (int e = 0; e < W; e++) bias[e] = k + q * W + e < cols_here ? __half2float(b[e]) : 0.0f;
+                    }
+                  }
+                  if (p.fe.aux) Pack16<__half>::widen(ld_shared_v4(out_buf + at), aux);
+                  fused_values<kCode, true, W>(x, bias, aux, z);
+                  if constexpr (kCode < kGradCode)
+                    if (p.fe.pre) {
+                      const uint4 u = Pack16<__half>::narrow(z);
+                      st_shared_v4(pre_buf + at, u.x, u.y, u.z, u.w);
+                    }
+                  const uint4 u = Pack16<__half>::narrow(x);
+                  st_shared_v4(out_buf + at, u.x, u.y, u.z, u.w);
+                }
+              }
               fence_proxy_async_smem();
               __syncwarp();
-              const int64_t col = n0h + c + 32 - COLS_PER_BUF;
-              if (store_leader) {
-                if (m_warp < p.M && col < p.N) tma_store_3d(&mapC.m[0], buf, (int)col, m_warp, (int)t.mat);
-                bulk_commit();
+              const bool live = rows_here > 0 && cols_here > 0;
+              if (ring_tma) {
+                if (store_leader) {
+                  if (kCode < kGradCode && p.fe.pre) {
+                    if (live) tma_store_3d(&mapC.m[1], pre_buf, (int)col0, m_warp, 0);
+                    bulk_commit();
+                  }
+                  if (live) tma_store_3d(&mapC.m[0], out_buf, (int)col0, m_warp, 0);
+                  bulk_commit();
+                  if (aux_tma) {
+                    // The block two uses on goes into the buffer of the use before this one, once that one's store has
+                    // read it: two passes ahead, or one where the pre-activation takes a use of its own.
+                    bulk_wait_read<1>();
+                    fetch_aux(ring_use + 2, tile, c / 64 + aux_ahead);
+                  }
+                }
+              } else if (live) {
+                if (kCode < kGradCode && p.fe.pre)
+                  block_to_memory<__half>(pre_buf, (__half*)p.fe.pre + (int64_t)m_warp * p.ldc + col0, p.ldc, rows_here, cols_here);
+                block_to_memory<__half>(out_buf, (__half*)p.C + (int64_t)m_warp * p.ldc + col0, p.ldc, rows_here, cols_here);
               }
+              ring_use++;
+              ring_pass++;
             }
+          });
+          if (!ok) {
+            if (lane == 0) { atomicOr(p.status, kDevTimeoutEpilogue); abort_flag = 1; }
+            break;
           }
         } else if (tma_store) {
           // Each warp rounds its 32 rows x 128 bytes into a swizzled staging buffer and one lane
           // sends it with a TMA store (full 128-byte lines); two buffers per warp alternate.
           constexpr int COLS_PER_BUF = kOutHalf ? 64 : 32;   // columns in one 128-byte staging row
           constexpr int LOADS = STG_BUFS * (kOutHalf ? 2 : 1);   // tcgen05.ld.x32 per pass (all staging buffers)
-          static_assert(COLS_PER_PART % (STG_BUFS * COLS_PER_BUF) == 0, "a pass fills every staging buffer");
+          static_assert(kRing || COLS_PER_PART % (STG_BUFS * COLS_PER_BUF) == 0, "a pass fills every staging buffer");
           const int m_warp = (int)(gm - lane);
           const uint32_t row_addr = stg_base + (uint32_t)lane * 128u;
           const uint32_t sw = (uint32_t)(lane & 7);
@@ -1198,9 +1368,7 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
             float v[32];
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = __uint_as_float(r[j]);
-            if (kMode == kFused)
-              fused_row32<OutT>(p.fe, row_off + n0h + c, n0h + c, gm < p.M ? p.N - n0h - c : 0, v);
-            else if (p.bias)
+            if (p.bias)
               add_bias<kOutHalf, 32>(p.bias, n0h + c, p.N, v);
             if (gm < row_end && n0h + c < p.N) store_row32<kOutHalf>(cmat, row_off, n0h + c, p.N, v, p.vec_ok != 0);
           }
@@ -1238,32 +1406,31 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
           mbar_arrive_cluster_relaxed(tempty_leader + 8 * slot);
           win++;
         }
-        if (kMode == kFused && ok) {
-          // 32 columns at a time go through the warp's staging buffer as they are, so that the epilogue's
-          // arithmetic, which picks them up chunk by chunk, need not be unrolled over the registers.
-          const int m_warp = t.tm * (BM * kCta) + (int)rank * BM + quarter * 32;
-          const uint32_t row_addr = stg_base + (uint32_t)lane * 128u;
+        if (kMode == kFused) {
+          // 32 columns at a time go through the warp's staging buffer as they are, so that the epilogue's arithmetic, which
+          // picks them up chunk by chunk in fused_block, need not be unrolled over the registers.
           const uint32_t sw = (uint32_t)(lane & 7);
 #pragma unroll
-          for (int c = 0; c < COLS_PER_THREAD; c += 32) {
-            if (p.tma_store && store_leader) bulk_wait_read<0>();
+          for (int c = 0; c < COLS_PER_THREAD && ok; c += 32) {
+            if (store_leader) bulk_wait_read<0>();
             __syncwarp();
+            uint4 aux[8];
+            const int m_warp = (int)(gm - lane);
+            const int rows_here = (int)min((int64_t)32, p.M - m_warp), cols_here = (int)min((int64_t)32, p.N - n0 - c);
+            if (rows_here <= 0 || cols_here <= 0) continue;
+            const int64_t at = (int64_t)m_warp * p.ldc + n0 + c;
+            if (p.fe.aux) {   // turned through the buffer: read a row at a time, needed a row a lane
+              block_from_memory<float>(stg_base, (const float*)p.fe.aux + at, p.ldc, rows_here, cols_here);
+              __syncwarp();
+#pragma unroll
+              for (int q = 0; q < 8; q++) aux[q] = ld_shared_v4(stg_base + (uint32_t)lane * 128u + (((uint32_t)q ^ sw) << 4));
+              __syncwarp();
+            }
 #pragma unroll
             for (int q = 0; q < 8; q++)
-              st_shared_v4(row_addr + (((uint32_t)q ^ sw) << 4), __float_as_uint(acc[c + q * 4]), __float_as_uint(acc[c + q * 4 + 1]),
-                           __float_as_uint(acc[c + q * 4 + 2]), __float_as_uint(acc[c + q * 4 + 3]));
-            const int64_t left = gm < p.M ? p.N - n0 - c : 0;
-            uint4 aux[8];
-            load_aux<float>(p.fe, row_off + n0 + c, left, aux);
-            fused_staged32(p, row_addr, sw, row_off + n0 + c, n0 + c, left, aux);
-            if (p.tma_store) {
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (store_leader && m_warp < p.M && n0 + c < p.N) {
-                tma_store_3d(&mapC.m[0], stg_base, (int)(n0 + c), m_warp, (int)t.mat);
-                bulk_commit();
-              }
-            }
+              st_shared_v4(stg_base + (uint32_t)lane * 128u + (((uint32_t)q ^ sw) << 4), __float_as_uint(acc[c + q * 4]),
+                           __float_as_uint(acc[c + q * 4 + 1]), __float_as_uint(acc[c + q * 4 + 2]), __float_as_uint(acc[c + q * 4 + 3]));
+            fused_block(p, mapC, stg_base, aux, m_warp, (int)(n0 + c), rows_here, cols_here, store_leader);
           }
         } else if (ok && tma_store) {
           // Same staging as above, fed from the register accumulators: one buffer, 32 columns per pass.
@@ -1546,7 +1713,7 @@ template <int kElemBytes, int kBN, int kStages, int kEpiWarps, bool kWindowed, i
 struct TcConfig {
   // operand ring (float32 slots also hold the lo slabs) + store staging + alignment slack
   static constexpr size_t smem = (size_t)kStages * kSlabs * (kElemBytes == 4 ? 2 : 1) * (BM * 128 + kNSplit * (kBN / kCta) * 128) +
-                                 (size_t)kEpiWarps * staging_bufs((kElemBytes == 2 && !kPartial) ? 2 : 4, kBN, kEpiWarps, kWindowed, kNSplit) * 4096 + 1024;
+                                 (size_t)kEpiWarps * (staging_ring(kMode, kWindowed) ? 3 : staging_bufs((kElemBytes == 2 && !kPartial) ? 2 : 4, kBN, kEpiWarps, kWindowed, kNSplit)) * 4096 + 1024;
   static_assert(smem <= 232448, "more shared memory than one CTA can have on sm_100");
   static constexpr int block = 96 + 32 * kEpiWarps;   // producers A and B, MMA issuer, epilogue warps
   static auto kernel() { return tc_gemm_kernel<kElemBytes, kBN, kStages, kEpiWarps, kWindowed, kCta, kNSplit, kSlabs, kPartial, kMode>; }
