@@ -51,13 +51,14 @@ class DType(enum.Enum):
 
     @property
     def byteSize(self) -> int:
-        return {"float16": 2, "float32": 4, "int64": 8}[self.value]
+        return _BYTE_SIZE[self._value_]
 
     @property
     def numpy(self):
         return {"float16": np.float16, "float32": np.float32, "int64": np.int64}[self.value]
 
 
+_BYTE_SIZE = {"float16": 2, "float32": 4, "int64": 8}
 _DTYPE_OF = {}
 
 
@@ -586,12 +587,21 @@ class CUDABackend:
         """(address, object to keep alive) of an input of `count` elements; None stays null."""
         if x is None:
             return None, None
-        if not isinstance(x, (CUDAData, np.ndarray)) and hasattr(x, "element_size"):
-            if _torch_dtype(x.dtype) is not dt:
+        if type(x) is CUDAData:
+            if x.byteCount < count * dt.byteSize:
+                raise ValueError(f"{what} is smaller than its {count} elements")
+            return x.ptr, x
+        if hasattr(x, "element_size"):   # a torch tensor
+            if _TORCH_DTYPE.get(x.dtype) is not dt and _torch_dtype(x.dtype) is not dt:
                 raise ValueError(f"{what} has type {x.dtype}, not {dt.value}")
-            if x.device.index != self.device:
+            if x.get_device() != self.device:   # -1 on the host
                 raise ValueError(f"{what} lies on {x.device}, the backend on device {self.device}")
-        elif isinstance(x, np.ndarray) and x.dtype != dt.numpy:
+            if not x.is_contiguous():
+                raise ValueError(f"{what}: torch operands must be contiguous CUDA tensors")
+            if x.numel() < count:
+                raise ValueError(f"{what} is smaller than its {count} elements")
+            return x.data_ptr(), x
+        if isinstance(x, np.ndarray) and x.dtype != dt.numpy:
             raise ValueError(f"{what} has type {x.dtype}, not {dt.value}")
         ptr, n, keep = self._operand(x, dt)
         if n < count * dt.byteSize:

@@ -282,6 +282,9 @@ cudaError_t launch_grouped(const GroupedProblem& p, cudaStream_t stream, unsigne
   maps[1] = maps[0]; maps[3] = maps[2];
   if (f32 && (!operand(&maps[1], a.lo, a, a.ld, a.rows * a.ld, a_mn, BM) || !operand(&maps[3], b.lo, b, b.ld, b.rows * b.ld, b_mn, bn / cta)))
     return cudaErrorNotSupported;
+  if (!wg && (!operand(&outs.m[5], a.hi, a, a.hi_ld, a.hi_stride, false, kShortBox) ||
+              (f32 && !operand(&outs.m[6], a.lo, a, a.ld, a.rows * a.ld, false, kShortBox))))
+    return cudaErrorNotSupported;
   if (wg)
     for (int i = 0; i < 4; i++) {
       if (!tails[i]) continue;
@@ -299,6 +302,7 @@ cudaError_t launch_grouped(const GroupedProblem& p, cudaStream_t stream, unsigne
   tp.C = p.out; tp.ldc = n; tp.strideC = m * n;
   tp.status = status_word;
   tp.n_out = 1;
+  tp.a_box_rows = BM;
   tp.vec_ok = (((uintptr_t)p.out & 15) == 0 && (n * eb) % 16 == 0 && (out_mats == 1 || (m * n * eb) % 16 == 0)) ? 1 : 0;
   tp.tma_store = tp.vec_ok && n * eb < (1ll << 40) && make_output_map(&outs.m[0], p.out, eb, n, m, n, m * n, out_mats) ? 1 : 0;
   tp.groups = GroupTable{start, end, first_tile, (int)p.groups, wg ? 1 : 0};

@@ -464,13 +464,17 @@ cudaError_t prepare_tc(const GemmProblem& p, unsigned int* status_word, void* sc
   const int bn = (shape == SHAPE_C1_128 || shape == SHAPE_PAIR_128) ? 128 : shape == SHAPE_PAIR_64 ? 64 : 256;
   const int cta = (shape == SHAPE_C1_256 || shape == SHAPE_C1_128) ? 1 : 2;
   const int b_box = bn / cta;
+  // A fused product of few rows copies those rows only: 128-row boxes of rows that are mostly not there cost the copies of the
+  // others their time (16384 x 4096 float16 weights, 4 rows: 46 us, 26 with 8-row boxes).
+  int a_box = BM;
+  if (p.fused && !p.a_mn_major && cta == 1 && p.M <= 64) a_box = p.M <= 8 ? 8 : p.M <= 16 ? 16 : p.M <= 32 ? 32 : 64;
   memset(pp.maps, 0, sizeof pp.maps);
   memset(&pp.outs, 0, sizeof pp.outs);
-  if (!make_operand_map(&pp.maps[0], a_hi, eb, p.a_mn_major, p.M, p.K, lda, sa, p.batch, BM) ||
+  if (!make_operand_map(&pp.maps[0], a_hi, eb, p.a_mn_major, p.M, p.K, lda, sa, p.batch, a_box) ||
       !make_operand_map(&pp.maps[2], b_hi, eb, p.b_mn_major, p.N, p.K, ldb, sb, p.batch, b_box))
     return cudaErrorNotSupported;
   if (f32) {
-    if (!make_operand_map(&pp.maps[1], a_lo, eb, p.a_mn_major, p.M, p.K, lda_lo, sa_lo, p.batch, BM) ||
+    if (!make_operand_map(&pp.maps[1], a_lo, eb, p.a_mn_major, p.M, p.K, lda_lo, sa_lo, p.batch, a_box) ||
         !make_operand_map(&pp.maps[3], b_lo, eb, p.b_mn_major, p.N, p.K, ldb_lo, sb_lo, p.batch, b_box))
       return cudaErrorNotSupported;
   } else {
@@ -516,6 +520,7 @@ cudaError_t prepare_tc(const GemmProblem& p, unsigned int* status_word, void* sc
   int out_bytes = eb;
   int64_t out_ld = p.ldc, out_stride = p.strideC, out_mats = p.batch;
   tp.bias = p.bias;
+  tp.a_box_rows = a_box;
   tp.fe = p.fe;
   // 16-byte accesses to the tensors laid out like the result
   tp.fe.vec = ((((uintptr_t)p.fe.aux | (uintptr_t)p.fe.pre) & 15) == 0 && (p.ldc * eb) % 16 == 0) ? 1 : 0;
@@ -684,6 +689,21 @@ cudaError_t issue_tc(const TcPrepared& pp, int sm_count, cudaStream_t stream, La
 }
 
 }  // namespace
+
+cudaError_t launch_sum_parts(const GemmProblem& p, const float* ws, int64_t ws_ld, int parts, cudaStream_t stream) {
+  ReduceJob job;
+  job.ws = ws; job.C = p.C; job.bias = nullptr;
+  job.M = p.M; job.N = p.N; job.ws_ld = ws_ld; job.batch = 1; job.parts = parts;
+  job.ldc = p.ldc; job.strideC = p.strideC;
+  job.fe = p.fe;
+  const bool f32 = p.dtype == HC_F32;
+  job.vec_ok = (((uintptr_t)p.C & (f32 ? 15 : 7)) == 0 && p.ldc % 4 == 0) ? 1 : 0;
+  int64_t blocks = (p.M * (ws_ld / 4) + 255) / 256;
+  if (blocks > 148 * 8) blocks = 148 * 8;
+  void* args[1] = {(void*)&job};
+  return launch_elementwise(f32 ? (const void*)splitk_reduce_kernel<false, true> : (const void*)splitk_reduce_kernel<true, true>, args,
+                            (int)blocks, stream);
+}
 
 void tc_forget_predecessor(cudaStream_t stream) {
   std::lock_guard<std::mutex> lock(g_track_mu);

@@ -285,7 +285,18 @@ hc_status run_problem(hc_ctx* ctx, hc_kernel kernel, const hc::GemmProblem& p, i
   }
   TraceScope trace(ctx, p);
   cudaError_t e;
-  if (chosen == HC_KERNEL_TENSOR) {
+  if (kernel == HC_KERNEL_AUTO && hc::skinny_fits(p) && (chosen != HC_KERNEL_TENSOR || hc::skinny_preferred(p))) {
+    size_t need = 0;
+    e = hc::launch_skinny(p, ctx->stream, ctx->scratch, ctx->scratch_bytes, ctx->sm_count, &ctx->last, &need);
+    if (e == cudaErrorInvalidValue && need > ctx->scratch_bytes) {
+      const hc_status st = ensure_scratch(ctx, need);
+      if (st != HC_OK) return st;
+      hc::tc_cache_clear(ctx->cache);   // prepared launches point into the old work area
+      e = hc::launch_skinny(p, ctx->stream, ctx->scratch, ctx->scratch_bytes, ctx->sm_count, &ctx->last, &need);
+    }
+    if (e == cudaSuccess && !ctx->scratch_in_graph) ctx->scratch_in_graph = is_capturing(ctx);
+    hc::tc_forget_predecessor(ctx->stream);
+  } else if (chosen == HC_KERNEL_TENSOR) {
     if (!hc::tc_supported(p))
       return fail(ctx, HC_ERR_NOT_IMPLEMENTED, "product too large for the tensor-core kernel's 32-bit tile coordinates");
     hc_status st;

@@ -88,6 +88,9 @@ struct GroupTable {
   int count;
   int weight_grad;         // the groups' rows are the contracted index (else the result's rows)
 };
+// Rows of A that a copy brings for a tile with few of them: the accumulator rows behind get whatever the slot held before, and
+// are never stored.
+constexpr int kShortBox = 16;
 
 struct TcParams {
   int64_t M, N;
@@ -107,6 +110,7 @@ struct TcParams {
   int tma_store;      // results leave through shared memory and TMA stores (else direct stores)
   const void* bias;   // optional row vector added to the rounded product (Linear), or null
   int n_out;          // destinations of every result tile: this device's result, then peers' copies
+  int a_box_rows;       // rows of a K-major A that one copy brings (128 but for products of few rows)
   FusedEpilogue fe;     // kMode == kFused only
   GroupTable groups;    // kMode == kGrouped only
   int skip_input_wait;  // the operands are known not to be written by the kernel launched just before
@@ -838,12 +842,14 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
       // The ring starts empty: the first kStages slots of the first tile need no wait, and their
       // byte counts can be announced before the previous kernel is waited for.
       const int free_slots = (kMode != kGrouped && tile_first < p.total_tiles) ? min(kStages, kr.count) : 0;
+      uint32_t stage_tx = kCta * kSlabs * PARTS * ((uint32_t)p.a_box_rows * 128u + B_BYTES);
       if (do_a && rank == 0)
-        for (int i = 0; i < free_slots; i++) mbar_expect_tx(bar_full + 8 * i, STAGE_BYTES * kCta);
+        for (int i = 0; i < free_slots; i++) mbar_expect_tx(bar_full + 8 * i, stage_tx);
       if (kMode != kGrouped && !p.skip_input_wait) pdl_wait();
       for (int64_t tile = tile_first; ok && tile < total_tiles; tile += tile_step) {
         if (kMode != kGrouped && tile != tile_first) { t = decode_tile(tile, p); kr = k_range(t.mat, p); }
         int a_row0 = 0, k_row0 = 0, whole_slabs = 0, tail_row = 0, b_mat = kr.mat;
+        bool short_a = false;
         if (kMode == kGrouped) {
           const GroupTile gt = decode_group_tile(tile, p);
           t.tm = gt.tm; t.tn = gt.tn;
@@ -859,6 +865,14 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
             whole_slabs = nkb;   // K's own end is the tensor's, which fills zeros
             a_row0 = gt.start;
             b_mat = gt.g;
+            // few rows of the group in this CTA's part of the tile (and in the partner's: the leader announces both)
+            stage_tx = 0;
+#pragma unroll
+            for (int r = 0; r < kCta; r++) {
+              const bool few = gt.n - gt.tm * (BM * kCta) - r * BM <= kShortBox;
+              if (r == (int)rank) short_a = few;
+              stage_tx += PARTS * ((few ? kShortBox : BM) * 128u + B_BYTES);
+            }
           }
           kr.mat = 0;
         }
@@ -876,7 +890,7 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
           const uint32_t full = full_leader + 8 * s;
           // (copies of B may complete before the bytes are announced: the count goes negative
           // for a moment, and the phase cannot complete before this arrive)
-          if (rank == 0 && do_a && kb >= prearmed) mbar_expect_tx(bar_full + 8 * s, STAGE_BYTES * kCta);
+          if (rank == 0 && do_a && kb >= prearmed) mbar_expect_tx(bar_full + 8 * s, stage_tx);
           // A slab past the end of K lies outside the tensor and arrives as zeros.
 #pragma unroll
           for (int j = 0; j < kSlabs; j++) {
@@ -889,6 +903,7 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
             const CUtensorMap* ma = part ? &mapA_lo : &mapA_hi;
             const CUtensorMap* mb = part ? &mapB_lo : &mapB_hi;
             if (tail) { ma = &mapC.m[1 + part]; mb = &mapC.m[3 + part]; }
+            if (kMode == kGrouped && short_a) ma = &mapC.m[5 + part];
             const uint32_t sa = stage + part * A_BYTES, sb = stage + PARTS * A_BYTES + part * B_BYTES;
             if (do_a) {
               if (!p.a_mn_major) {
@@ -1198,7 +1213,7 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
           // enters (the auxiliary tensor, whose block the result then overwrites) takes the next of three buffers; a
           // block's own bulk group tells when its buffer has been read.  Auxiliary blocks are fetched ahead.
           // The loops are rolled and exist once for every kind of epilogue: unrolled over a tile with the choice inside,
-          // their code outgrew the instruction cache (8192 x 512 x 8192, no extras: 109 us against RINGNONE).
+          // their code outgrew the instruction cache (8192 x 512 x 8192, no extras: 109 us against 74).
           constexpr int W = 8;
           static_assert(!kRing || COLS_PER_PART % 64 == 0, "whole passes");
           const uint32_t sw = (uint32_t)(lane & 7);
@@ -1526,6 +1541,22 @@ __device__ __forceinline__ float split_lo(float x) {
   return __uint_as_float(lbits & 0xFFFFE000u);
 }
 
+// Element i of rows of `width`, of `total` elements: by 32-bit division where that suffices (the usual case; 64-bit division
+// was most of these kernels' instructions).
+struct RowOf { int64_t row, col; };
+__device__ __forceinline__ RowOf row_of(int64_t i, int64_t width, int64_t total) {
+  RowOf a;
+  if (total < (1ll << 32)) {
+    const uint32_t r = (uint32_t)i / (uint32_t)width;
+    a.row = r;
+    a.col = (uint32_t)i - r * (uint32_t)width;
+  } else {
+    a.row = i / width;
+    a.col = i - a.row * width;
+  }
+  return a;
+}
+
 // One launch splits both operands: the first `blocks_a` blocks work on A, the rest on B.
 __global__ void __launch_bounds__(256) split_tf32_kernel(const SplitJob ja, const SplitJob jb, int blocks_a) {
   pdl_release();
@@ -1537,7 +1568,8 @@ __global__ void __launch_bounds__(256) split_tf32_kernel(const SplitJob ja, cons
   if (j.vec4) {
     const int64_t w4 = j.width / 4, total = j.batch * j.rows * w4;
     for (int64_t i = bid * blockDim.x + threadIdx.x; i < total; i += nblk * blockDim.x) {
-      const int64_t c = (i % w4) * 4, r = (i / w4) % j.rows, b = i / (w4 * j.rows);
+      const RowOf at = row_of(i, w4, total);
+      const int64_t c = at.col * 4, b = j.batch == 1 ? 0 : at.row / j.rows, r = at.row - b * j.rows;
       const float4 x = *(const float4*)(j.src + b * j.stride_src + r * j.ld_src + c);
       if (j.hi) *(float4*)(j.hi + b * j.stride_dst + r * j.ld_dst + c) = x;
       *(float4*)(j.lo + b * j.stride_dst + r * j.ld_dst + c) =
@@ -1546,7 +1578,8 @@ __global__ void __launch_bounds__(256) split_tf32_kernel(const SplitJob ja, cons
   } else {
     const int64_t total = j.batch * j.rows * j.width;
     for (int64_t i = bid * blockDim.x + threadIdx.x; i < total; i += nblk * blockDim.x) {
-      const int64_t c = i % j.width, r = (i / j.width) % j.rows, b = i / (j.width * j.rows);
+      const RowOf at = row_of(i, j.width, total);
+      const int64_t c = at.col, b = j.batch == 1 ? 0 : at.row / j.rows, r = at.row - b * j.rows;
       const float x = j.src[b * j.stride_src + r * j.ld_src + c];
       if (j.hi) j.hi[b * j.stride_dst + r * j.ld_dst + c] = x;
       j.lo[b * j.stride_dst + r * j.ld_dst + c] = split_lo(x);
@@ -1570,7 +1603,8 @@ __global__ void __launch_bounds__(256) repack_f16_kernel(const RepackJob ja, con
   const int64_t nblk = is_a ? blocks_a : (int64_t)gridDim.x - blocks_a;
   const int64_t total = j.batch * j.rows * j.width;
   for (int64_t i = bid * blockDim.x + threadIdx.x; i < total; i += nblk * blockDim.x) {
-    const int64_t c = i % j.width, r = (i / j.width) % j.rows, b = i / (j.width * j.rows);
+    const RowOf at = row_of(i, j.width, total);
+    const int64_t c = at.col, b = j.batch == 1 ? 0 : at.row / j.rows, r = at.row - b * j.rows;
     j.dst[b * j.stride_dst + r * j.ld_dst + c] = j.src[b * j.stride_src + r * j.ld_src + c];
   }
 }
