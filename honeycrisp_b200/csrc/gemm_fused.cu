@@ -7,11 +7,9 @@ namespace hc {
 TcLaunchFn fused_kernel(bool f32, int shape) {
   if (f32) {
     switch (shape) {
-      case SHAPE_PAIR_128: return TcConfig<4, 128, 3, 4, true, 2, 1, 1, false, kFused>::launch;
-      case SHAPE_PAIR_64: return TcConfig<4, 64, 4, 4, true, 2, 1, 1, false, kFused>::launch;
-      case SHAPE_PAIR: return TcConfig<4, 256, 3, 8, true, 2, 1, 1, false, kFused>::launch;
-      case SHAPE_C1_256: return TcConfig<4, 256, 2, 8, true, 1, 1, 1, false, kFused>::launch;
-      case SHAPE_C1_128: return TcConfig<4, 128, 3, 4, true, 1, 1, 1, false, kFused>::launch;
+      case SHAPE_PAIR_128: return TcConfig<4, 128, 4, 8, true, 2, 1, 1, false, kFused>::launch;
+      case SHAPE_PAIR_64: return TcConfig<4, 64, 4, 8, true, 2, 1, 1, false, kFused>::launch;
+      case SHAPE_C1_128: return TcConfig<4, 128, 3, 8, true, 1, 1, 1, false, kFused>::launch;
       default: return nullptr;
     }
   }

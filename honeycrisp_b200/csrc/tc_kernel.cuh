@@ -529,7 +529,8 @@ __device__ __noinline__ void block_to_memory(uint32_t buf, T* base, int64_t ld, 
       if (lane * V + e < cols) base[r * ld + lane * V + e] = v[e];
   }
 }
-// Into a staging block; the loads of many rows are under way before the first is needed.
+// Into a staging block; the loads of many rows are under way before the first is needed.  float32 arrives by asynchronous copies,
+// which the caller waits for.
 template <typename T>
 __device__ __noinline__ void block_from_memory(uint32_t buf, const T* base, int64_t ld, int rows, int cols) {
   const int lane = threadIdx.x & 31;
@@ -538,7 +539,6 @@ __device__ __noinline__ void block_from_memory(uint32_t buf, const T* base, int6
       for (int r = 0; r < rows; r++)
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(buf + r * 128 + ((uint32_t)((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4),
                      "l"(base + r * ld + lane) : "memory");
-    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     for (int r0 = 0; r0 < rows; r0 += 16) {
       uint32_t u[16];
@@ -639,61 +639,6 @@ __device__ __forceinline__ KRange k_range(int64_t vmat, const TcParams& p) {
     r.count = min(p.kb_per_split, p.num_k_blocks - r.kb0);
   }
   return r;
-}
-
-// The fused epilogue over a float32 staging block: every lane works on its own row's chunks, in place; where z is kept, the
-// block leaves once before the activation and once behind it.
-__device__ __noinline__ void fused_block(const TcParams& p, const OutMaps& mapC, uint32_t buf, const uint4 (&aux)[8], int row, int col,
-                                         int rows_here, int cols_here, bool store_leader) {
-  const int lane = threadIdx.x & 31;
-  const uint32_t sw = (uint32_t)(lane & 7);
-  const bool tma = p.tma_store && p.fe.vec;
-  auto leave = [&](const CUtensorMap* map, void* base) {
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (tma) {
-      if (store_leader) {
-        tma_store_3d(map, buf, col, row, 0);
-        bulk_commit();
-      }
-    } else {
-      block_to_memory<float>(buf, (float*)base + (int64_t)row * p.ldc + col, p.ldc, rows_here, cols_here);
-    }
-  };
-  if (!p.fe.grad && p.fe.bias) {
-#pragma unroll 1
-    for (int q = 0; q < 8; q++) {
-      const uint32_t at = buf + (uint32_t)lane * 128u + (((uint32_t)q ^ sw) << 4);
-      float x[4];
-      Pack16<float>::widen(ld_shared_v4(at), x);
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (q * 4 + e < cols_here) x[e] += __ldg((const float*)p.fe.bias + col + q * 4 + e);
-      const uint4 u = Pack16<float>::narrow(x);
-      st_shared_v4(at, u.x, u.y, u.z, u.w);
-    }
-  }
-  if (p.fe.pre) {
-    leave(&mapC.m[1], p.fe.pre);
-    if (tma && store_leader) bulk_wait_read<0>();
-    __syncwarp();
-  }
-  with_code(p.fe.act, p.fe.grad, [&](auto code) {
-    constexpr int kCode = decltype(code)::value;
-#pragma unroll 1
-    for (int q = 0; q < 8; q++) {
-      const uint32_t at = buf + (uint32_t)lane * 128u + (((uint32_t)q ^ sw) << 4);
-      const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      float x[4], a[4] = {0.0f, 0.0f, 0.0f, 0.0f}, z[4];
-      Pack16<float>::widen(ld_shared_v4(at), x);
-      if (p.fe.aux) Pack16<float>::widen(aux[q], a);
-      fused_values<kCode, false, 4>(x, none, a, z);
-      const uint4 u = Pack16<float>::narrow(x);
-      st_shared_v4(at, u.x, u.y, u.z, u.w);
-    }
-  });
-  leave(&mapC.m[0], p.C);
-  __syncwarp();
 }
 
 // kElemBytes: 2 (float16 operands) or 4 (float32 operands consumed as TF32).
@@ -1394,6 +1339,11 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
         win++;
       } else {
         float acc[COLS_PER_THREAD];
+        if (kMode == kFused && p.fe.aux) {   // the first block's auxiliary values travel under the main loop
+          const int rows_here = (int)min((int64_t)32, p.M - (gm - lane)), cols_here = (int)min((int64_t)32, p.N - n0);
+          if (rows_here > 0 && cols_here > 0)
+            block_from_memory<float>(stg_base, (const float*)p.fe.aux + (gm - lane) * p.ldc + n0, p.ldc, rows_here, cols_here);
+        }
         for (int w = 0; w < nwin && ok; w++) {
           const uint32_t slot = win & 1;
           const bool got = mbar_wait_warp(bar_tfull + 8 * slot, (win >> 1) & 1, abortp, lane);
@@ -1421,32 +1371,65 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
           mbar_arrive_cluster_relaxed(tempty_leader + 8 * slot);
           win++;
         }
-        if (kMode == kFused) {
-          // 32 columns at a time go through the warp's staging buffer as they are, so that the epilogue's arithmetic, which
-          // picks them up chunk by chunk in fused_block, need not be unrolled over the registers.
+        if constexpr (kMode == kFused) {
+          // 32 columns at a time: the auxiliary tensor's block, read into the staging buffer a row at a time, is picked up a row
+          // a lane and its place taken by z, where that is kept, and then by the result.
+          const uint32_t own_row = stg_base + (uint32_t)lane * 128u;
           const uint32_t sw = (uint32_t)(lane & 7);
+          const bool leave_tma = p.tma_store && p.fe.vec;
+          with_code(p.fe.act, p.fe.grad, [&](auto code) {
+            constexpr int kCode = decltype(code)::value;
+            auto leave = [&](const float (&v)[COLS_PER_THREAD], int c, const CUtensorMap* map, void* base, int rows_here, int cols_here) {
 #pragma unroll
-          for (int c = 0; c < COLS_PER_THREAD && ok; c += 32) {
-            if (store_leader) bulk_wait_read<0>();
-            __syncwarp();
-            uint4 aux[8];
-            const int m_warp = (int)(gm - lane);
-            const int rows_here = (int)min((int64_t)32, p.M - m_warp), cols_here = (int)min((int64_t)32, p.N - n0 - c);
-            if (rows_here <= 0 || cols_here <= 0) continue;
-            const int64_t at = (int64_t)m_warp * p.ldc + n0 + c;
-            if (p.fe.aux) {   // turned through the buffer: read a row at a time, needed a row a lane
-              block_from_memory<float>(stg_base, (const float*)p.fe.aux + at, p.ldc, rows_here, cols_here);
+              for (int q = 0; q < 8; q++)
+                st_shared_v4(own_row + (((uint32_t)q ^ sw) << 4), __float_as_uint(v[c + q * 4]), __float_as_uint(v[c + q * 4 + 1]),
+                             __float_as_uint(v[c + q * 4 + 2]), __float_as_uint(v[c + q * 4 + 3]));
+              fence_proxy_async_smem();
               __syncwarp();
+              if (leave_tma) {
+                if (store_leader) {
+                  tma_store_3d(map, stg_base, (int)(n0 + c), (int)(gm - lane), 0);
+                  bulk_commit();
+                  bulk_wait_read<0>();
+                }
+              } else {
+                block_to_memory<float>(stg_base, (float*)base + (gm - lane) * p.ldc + n0 + c, p.ldc, rows_here, cols_here);
+              }
+              __syncwarp();
+            };
 #pragma unroll
-              for (int q = 0; q < 8; q++) aux[q] = ld_shared_v4(stg_base + (uint32_t)lane * 128u + (((uint32_t)q ^ sw) << 4));
+            for (int c = 0; c < COLS_PER_THREAD; c += 32) {
+              const int rows_here = (int)min((int64_t)32, p.M - (gm - lane)), cols_here = (int)min((int64_t)32, p.N - n0 - c);
+              if (!ok || rows_here <= 0 || cols_here <= 0) continue;
+              if (p.fe.aux) {
+                if (c > 0) block_from_memory<float>(stg_base, (const float*)p.fe.aux + (gm - lane) * p.ldc + n0 + c, p.ldc, rows_here, cols_here);
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                __syncwarp();
+              }
+              float z[kCode < kGradCode ? COLS_PER_THREAD : 1];
+#pragma unroll
+              for (int q = 0; q < 8; q++) {
+                float x[4], bias[4], aux[4], zq[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                  x[e] = acc[c + q * 4 + e];
+                  aux[e] = 0.0f;
+                  bias[e] = kCode < kGradCode && p.fe.bias && q * 4 + e < cols_here ? __ldg((const float*)p.fe.bias + n0 + c + q * 4 + e) : 0.0f;
+                }
+                if (p.fe.aux) Pack16<float>::widen(ld_shared_v4(own_row + (((uint32_t)q ^ sw) << 4)), aux);
+                fused_values<kCode, false, 4>(x, bias, aux, zq);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                  acc[c + q * 4 + e] = x[e];
+                  if constexpr (kCode < kGradCode) z[c + q * 4 + e] = zq[e];
+                }
+              }
               __syncwarp();
+              if constexpr (kCode < kGradCode)
+                if (p.fe.pre) leave(z, c, &mapC.m[1], p.fe.pre, rows_here, cols_here);
+              leave(acc, c, &mapC.m[0], p.C, rows_here, cols_here);
             }
-#pragma unroll
-            for (int q = 0; q < 8; q++)
-              st_shared_v4(stg_base + (uint32_t)lane * 128u + (((uint32_t)q ^ sw) << 4), __float_as_uint(acc[c + q * 4]),
-                           __float_as_uint(acc[c + q * 4 + 1]), __float_as_uint(acc[c + q * 4 + 2]), __float_as_uint(acc[c + q * 4 + 3]));
-            fused_block(p, mapC, stg_base, aux, m_warp, (int)(n0 + c), rows_here, cols_here, store_leader);
-          }
+          });
         } else if (ok && tma_store) {
           // Same staging as above, fed from the register accumulators: one buffer, 32 columns per pass.
           const int m_warp = (int)(gm - lane);
@@ -1576,13 +1559,19 @@ __global__ void __launch_bounds__(256) split_tf32_kernel(const SplitJob ja, cons
           make_float4(split_lo(x.x), split_lo(x.y), split_lo(x.z), split_lo(x.w));
     }
   } else {
-    const int64_t total = j.batch * j.rows * j.width;
+    // Rows off 16-byte boundaries: four elements a thread, read one by one, written as one; the copies' pitch is a multiple of
+    // four, and what lies between a row's end and the next row's start is never read.
+    const int64_t w4 = (j.width + 3) / 4, total = j.batch * j.rows * w4;
     for (int64_t i = bid * blockDim.x + threadIdx.x; i < total; i += nblk * blockDim.x) {
-      const RowOf at = row_of(i, j.width, total);
-      const int64_t c = at.col, b = j.batch == 1 ? 0 : at.row / j.rows, r = at.row - b * j.rows;
-      const float x = j.src[b * j.stride_src + r * j.ld_src + c];
-      if (j.hi) j.hi[b * j.stride_dst + r * j.ld_dst + c] = x;
-      j.lo[b * j.stride_dst + r * j.ld_dst + c] = split_lo(x);
+      const RowOf at = row_of(i, w4, total);
+      const int64_t c = at.col * 4, b = j.batch == 1 ? 0 : at.row / j.rows, r = at.row - b * j.rows;
+      const float* src = j.src + b * j.stride_src + r * j.ld_src + c;
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] = c + e < j.width ? src[e] : 0.0f;
+      const int64_t to = b * j.stride_dst + r * j.ld_dst + c;
+      if (j.hi) *(float4*)(j.hi + to) = make_float4(x[0], x[1], x[2], x[3]);
+      *(float4*)(j.lo + to) = make_float4(split_lo(x[0]), split_lo(x[1]), split_lo(x[2]), split_lo(x[3]));
     }
   }
 }
@@ -1601,11 +1590,16 @@ __global__ void __launch_bounds__(256) repack_f16_kernel(const RepackJob ja, con
   const RepackJob& j = is_a ? ja : jb;
   const int64_t bid = is_a ? blockIdx.x : blockIdx.x - blocks_a;
   const int64_t nblk = is_a ? blocks_a : (int64_t)gridDim.x - blocks_a;
-  const int64_t total = j.batch * j.rows * j.width;
+  const int64_t w8 = (j.width + 7) / 8, total = j.batch * j.rows * w8;   // the copy's pitch is a multiple of eight
   for (int64_t i = bid * blockDim.x + threadIdx.x; i < total; i += nblk * blockDim.x) {
-    const RowOf at = row_of(i, j.width, total);
-    const int64_t c = at.col, b = j.batch == 1 ? 0 : at.row / j.rows, r = at.row - b * j.rows;
-    j.dst[b * j.stride_dst + r * j.ld_dst + c] = j.src[b * j.stride_src + r * j.ld_src + c];
+    const RowOf at = row_of(i, w8, total);
+    const int64_t c = at.col * 8, b = j.batch == 1 ? 0 : at.row / j.rows, r = at.row - b * j.rows;
+    const __half* src = j.src + b * j.stride_src + r * j.ld_src + c;
+    uint4 u;
+    __half* x = (__half*)&u;
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = c + e < j.width ? src[e] : __half(0.0f);
+    *(uint4*)(j.dst + b * j.stride_dst + r * j.ld_dst + c) = u;
   }
 }
 
