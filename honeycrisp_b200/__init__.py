@@ -3,7 +3,8 @@
 Public surface:
   CUDABackend, CUDAData, DType, BackendError (+ subclasses)  - honeycrisp_b200.backend
   Tensor, matmul, batchedMatmul                               - honeycrisp_b200.linalg
-  Linear (fused-bias forward, on-device backward)             - honeycrisp_b200.linear
+  Linear (fused forward, on-device backward)                  - honeycrisp_b200.linear
+  LayerNorm, FeedForward, Experts, AdamW                      - honeycrisp_b200.feedforward
   shardBatch, columnBlock, batchedMatmulSharded, matmulColumnSplit - honeycrisp_b200.sharding
 The compute library is honeycrisp_b200/libhccuda.so (C ABI in include/hc_cuda.h).
 """
@@ -11,8 +12,9 @@ from .backend import (AdamWPlan, AllocationFailed, BackendError, CUDABackend, CU
                       KernelFailed, NotImplementedByBackend)
 from .linalg import Tensor, batchedMatmul, matmul
 from .linear import Linear
+from .feedforward import AdamW, Experts, FeedForward, LayerNorm
 
 __all__ = [
-    "AdamWPlan", "AllocationFailed", "BackendError", "CUDABackend", "CUDAData", "DeviceTimeout", "DType", "KernelFailed",
-    "Linear", "NotImplementedByBackend", "Tensor", "batchedMatmul", "matmul",
+    "AdamW", "AdamWPlan", "AllocationFailed", "BackendError", "CUDABackend", "CUDAData", "DeviceTimeout", "DType", "Experts", "FeedForward",
+    "KernelFailed", "LayerNorm", "Linear", "NotImplementedByBackend", "Tensor", "batchedMatmul", "matmul",
 ]

@@ -256,14 +256,14 @@ class AdamWPlan:
     """The tensors of an AdamW step, laid out once for all steps (Adam of the reference's Optimizer.swift holds
     its parameters the same way).  Parameters and gradients are float16 or float32, moments float32; torch tensors
     bring their type and length, CUDAData needs `dtype` (and `gradDType`, if it differs) and `count` in its dict.  The plan keeps
-    the tensors alive; their addresses must stay what they are."""
+    the tensors alive; their addresses must stay what they are, but for a gradient's, which setGrad replaces."""
 
     def __init__(self, backend: "CUDABackend", tensors):
         tensors = list(tensors)
         self.count = len(tensors)
         self._table = (L.AdamWTensor * max(1, self.count))()
-        self._keep, self._updated = [], []
-        for row, t in zip(self._table, tensors):
+        self._backend, self._keep, self._grads, self._updated = backend, [], {}, []
+        for index, (row, t) in enumerate(zip(self._table, tensors)):
             if set(t) - {"param", "grad", "moment1", "moment2", "copy", "count", "dtype", "gradDType"}:
                 raise ValueError(f"AdamWPlan: unknown entries {sorted(t)}")
             p = t["param"]
@@ -279,11 +279,24 @@ class AdamWPlan:
                     raise TypeError(f"AdamWPlan: {name} must lie on the device")
                 ptr, keep = backend._input(x, dt, count, name)
                 setattr(row, name, ptr or None)
-                self._keep.append(keep)
+                if name == "grad":
+                    self._grads[index] = keep
+                else:
+                    self._keep.append(keep)
                 if name != "grad" and isinstance(x, CUDAData):
                     self._updated.append(x)
             row.count = count
             row.param_dtype, row.grad_dtype = _HC_DTYPE[pd], _HC_DTYPE[gd]
+
+    def setGrad(self, index: int, grad) -> None:
+        """Tensor `index` takes its gradient from `grad` (of the same type and length) from now on."""
+        row = self._table[index]
+        gd = DType.float16 if row.grad_dtype == L.HC_F16 else DType.float32
+        ptr, keep = self._backend._input(grad, gd, row.count, "grad")
+        if isinstance(grad, np.ndarray):
+            raise TypeError("AdamWPlan: grad must lie on the device")
+        row.grad = ptr or None
+        self._grads[index] = keep
 
     @staticmethod
     def _dtype(x, given) -> DType:

@@ -19,6 +19,14 @@ weights cast on every call); a float16 layer with a bias and no castParams adds 
 float32, which the reference's binary ops refuse, and so does this class.  Gradients arrive in the
 compute dtype and are cast back to each parameter's dtype (the backward of `cast`).
 
+With an activation or a residual the layer runs as one product with a fused epilogue instead,
+
+    pre = x . W + b,   out = activation(pre) + residual          (float32 throughout, rounded once)
+
+and its backward pass starts with the gradient through the activation, which brings the bias gradient along.  A layer in front of
+it can take its own activation's slope into this layer's input gradient (`inputPre`, `inputActivation`): the product
+dX = dPre . W^T then leaves as the gradient of that layer's pre-activation.
+
 Weights come from numpy's generator, not from Honeycrisp's Philox stream, so parameter values
 differ from a Honeycrisp `Linear` with the same seed; shapes, ranges and arithmetic do not.
 """
@@ -34,11 +42,12 @@ from .backend import CUDABackend, CUDAData, DType, _as_dtype
 
 class Linear:
     def __init__(self, backend: CUDABackend, inCount: int, outCount: int, dtype=np.float32, castParams=None,
-                 bias: bool = True, seed: int = 0):
+                 bias: bool = True, seed: int = 0, activation: Optional[str] = None):
         self.backend, self.inCount, self.outCount = backend, int(inCount), int(outCount)
         self.dtype = _as_dtype(dtype)                                    # of the weight
         self.castParams = _as_dtype(castParams) if castParams is not None else None
         self.biasDType = DType.float32                                   # Trainable.swift:524
+        self.activation = activation if activation != "none" else None
         rng = np.random.default_rng(seed)
         w = (rng.random((inCount, outCount), dtype=np.float32) - 0.5) * (math.sqrt(3.0) / 0.5 / math.sqrt(inCount))
         self.weight = backend.collection(w.astype(self.dtype.numpy), self.dtype)
@@ -68,32 +77,83 @@ class Linear:
             return self.bias
         return self.backend.cast(self.bias, self.outCount, self.biasDType, bt)
 
-    def __call__(self, x, shape: Sequence[int]) -> Tuple[CUDAData, list]:
+    def __call__(self, x, shape: Sequence[int], residual=None) -> Tuple[CUDAData, list]:
         """Forward.  `x` holds a dense tensor of `shape`, in the layer's compute dtype, whose last
-        dimension is inCount; returns the output buffer and its shape."""
+        dimension is inCount; returns the output buffer and its shape.  `residual`, of the output's shape, is added behind
+        the activation."""
+        if self.activation is None and residual is None:
+            shape, rows = self._rows(shape)
+            out = self.backend.linearForward(x, self._castWeight(), self._castBias(), rows, self.inCount, self.outCount,
+                                             self.computeDType)
+            return out, shape[:-1] + [self.outCount]
+        return self._fused(x, shape, residual, None)
+
+    def forwardKeepingPre(self, x, shape: Sequence[int], residual=None) -> Tuple[CUDAData, list, CUDAData]:
+        """Forward for training a layer with an activation: also returns the activation's input, for `backward`."""
+        _, rows = self._rows(shape)
+        pre = self.backend.allocate(rows * self.outCount * self.computeDType.byteSize)
+        out, outShape = self._fused(x, shape, residual, pre)
+        return out, outShape, pre
+
+    def _rows(self, shape):
         shape = list(int(s) for s in shape)
         assert shape and shape[-1] == self.inCount, f"last dimension must be {self.inCount}: {shape}"
-        rows = int(np.prod(shape[:-1])) if len(shape) > 1 else 1
-        out = self.backend.linearForward(x, self._castWeight(), self._castBias(), rows, self.inCount, self.outCount,
-                                         self.computeDType)
+        return shape, int(np.prod(shape[:-1])) if len(shape) > 1 else 1
+
+    def _fused(self, x, shape, residual, pre):
+        shape, rows = self._rows(shape)
+        out = self.backend.matmulEpilogue(x, False, self._castWeight(), False, rows, self.inCount, self.outCount, self.computeDType,
+                                          activation=self.activation, bias=self._castBias(), residual=residual, pre=pre)
         return out, shape[:-1] + [self.outCount]
 
-    def backward(self, x, shape: Sequence[int], outGrad) -> CUDAData:
+    def backward(self, x, shape: Sequence[int], outGrad, pre=None, inputPre=None, inputActivation: Optional[str] = None) -> CUDAData:
         """Backward for the forward call on (`x`, `shape`): returns dX and accumulates the
-        parameter gradients (Param.addGrad, Trainable.swift:258-266)."""
+        parameter gradients (Param.addGrad, Trainable.swift:258-266).  `pre` is what forwardKeepingPre returned, for a layer with
+        an activation (a residual's gradient is outGrad itself).  With `inputPre` and `inputActivation`, the input of this
+        layer is inputActivation(inputPre) and what comes back is the gradient of inputPre."""
         shape = list(int(s) for s in shape)
         rows = int(np.prod(shape[:-1])) if len(shape) > 1 else 1
         be = self.backend
         ct = self.computeDType
-        dx = be.matmul(outGrad, False, self._castWeight(), True, False, rows, self.outCount, self.inCount, ct)
+        db = None
+        if self.activation is not None:
+            if pre is None:
+                raise ValueError("Linear: the backward pass of a layer with an activation needs `pre` (forwardKeepingPre)")
+            outGrad, db = be.activationGrad(outGrad, pre, rows, self.outCount, ct, self.activation, biasGrad=self.bias is not None)
+        return self._backwardOfPre(x, rows, outGrad, db, inputPre, inputActivation)
+
+    def backwardOfPre(self, x, shape: Sequence[int], preGrad) -> CUDAData:
+        """Backward from the gradient of the activation's input, as the layer behind returns it (`inputPre`)."""
+        _, rows = self._rows(shape)
+        return self._backwardOfPre(x, rows, preGrad, None, None, None)
+
+    def _backwardOfPre(self, x, rows: int, outGrad, db, inputPre, inputActivation) -> CUDAData:
+        be = self.backend
+        ct = self.computeDType
+        if inputPre is not None:
+            dx = be.matmulEpilogue(outGrad, False, self._castWeight(), True, rows, self.outCount, self.inCount, ct,
+                                   activation=inputActivation, gradPre=inputPre)
+        else:
+            dx = be.matmul(outGrad, False, self._castWeight(), True, False, rows, self.outCount, self.inCount, ct)
         dw = be.matmul(x, True, outGrad, False, False, self.inCount, rows, self.outCount, ct)
         if ct != self.dtype:                          # backward of weight.cast(castParams)
             dw = be.cast(dw, self.inCount * self.outCount, ct, self.dtype)
         self.weightGrad = dw if self.weightGrad is None else be.add(self.weightGrad, dw, self.inCount * self.outCount,
                                                                     self.dtype)
         if self.bias is not None:
-            db = be.columnSum(outGrad, rows, self.outCount, ct)
-            if ct != self.biasDType:                  # backward of bias.cast(castParams)
-                db = be.cast(db, self.outCount, ct, self.biasDType)
+            if db is None:
+                db = be.columnSum(outGrad, rows, self.outCount, ct)
+                if ct != self.biasDType:              # backward of bias.cast(castParams)
+                    db = be.cast(db, self.outCount, ct, self.biasDType)
             self.biasGrad = db if self.biasGrad is None else be.add(self.biasGrad, db, self.outCount, self.biasDType)
         return dx
+
+    def parameters(self):
+        """(buffer, gradient, element count, dtype) of each parameter, for AdamW."""
+        out = [(self.weight, self.weightGrad, self.inCount * self.outCount, self.dtype)]
+        if self.bias is not None:
+            out.append((self.bias, self.biasGrad, self.outCount, self.biasDType))
+        return out
+
+    def zeroGrad(self) -> None:
+        self.weightGrad = self.biasGrad = None

@@ -1,0 +1,130 @@
+"""What the host refuses before anything reaches a device: the C entry points without a context, and the checks of the Python face."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from honeycrisp_b200 import _lib as L
+from honeycrisp_b200 import backend as B
+
+
+def test_entry_points_without_a_context():
+    lib = L.load()
+    ep = L.Epilogue(0, None, None, None, None)
+    bad = L.HC_ERR_INVALID_ARGUMENT
+    assert lib.hc_matmul_epilogue(None, L.HC_F16, None, 0, None, 0, 1, 1, 1, ctypes.byref(ep), None) == bad
+    assert lib.hc_activation_grad(None, L.HC_F16, 0, None, None, 1, 1, None, None) == bad
+    assert lib.hc_layer_norm(None, L.HC_F16, L.HC_F32, None, None, None, 1, 1, 1e-5, None, None, None) == bad
+    assert lib.hc_layer_norm_grad(None, L.HC_F16, L.HC_F32, None, None, None, None, None, 1, 1, None, None, None) == bad
+    assert lib.hc_grouped_matmul(None, L.HC_F16, 1, None, None, None, 0, 1, 1, 1, None) == bad
+    assert lib.hc_grouped_matmul_weight_grad(None, L.HC_F16, 1, None, None, None, 1, 1, 1, None) == bad
+    assert lib.hc_adamw(None, None, 0, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0) == bad
+
+
+class Recorder:
+    """A library whose calls succeed and are written down."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return L.HC_OK
+        return call
+
+
+@pytest.fixture
+def be():
+    b = B.CUDABackend.__new__(B.CUDABackend)
+    b._lib, b._ctx, b.device = Recorder(), 1, 0
+    yield b
+    b._ctx = None
+
+
+def data(be, elements, size=2):
+    return B.CUDAData(be, 256, elements * size, owns=False)
+
+
+def called(be, name):
+    return [a for n, a in be._lib.calls if n == name]
+
+
+def test_epilogue_passes_what_it_was_given(be):
+    a, b, bias, res, pre, out = data(be, 12), data(be, 20), data(be, 5), data(be, 15), data(be, 15), data(be, 15)
+    assert be.matmulEpilogue(a, False, b, True, 3, 4, 5, "float16", activation="silu", bias=bias, residual=res, pre=pre, out=out, mark=False) is out
+    (args,) = called(be, "hc_matmul_epilogue")
+    assert args[1] == L.HC_F16 and args[3] == 0 and args[5] == 1 and args[6:9] == (3, 4, 5)
+    assert out._inputs[2] is bias and out._inputs[3] is res
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(bias=4), "bias is smaller"), (dict(residual=14), "residual is smaller"), (dict(pre=14), "pre is smaller"),
+    (dict(gradPre=14), "gradPre is smaller"), (dict(out=14), "out is smaller"), (dict(activation="swish"), "unknown activation")])
+def test_epilogue_refuses(be, change, error):
+    change = {k: data(be, v) if isinstance(v, int) else v for k, v in change.items()}
+    change.setdefault("out", data(be, 15))
+    with pytest.raises(ValueError, match=error):
+        be.matmulEpilogue(data(be, 12), False, data(be, 20), False, 3, 4, 5, np.float16, **change)
+    with pytest.raises(ValueError, match="operand a"):
+        be.matmulEpilogue(data(be, 11), False, data(be, 20), False, 3, 4, 5, np.float16, out=data(be, 15))
+    assert not called(be, "hc_matmul_epilogue")
+
+
+def test_types_are_checked(be):
+    import torch
+    out = data(be, 16)
+    with pytest.raises(ValueError, match="type"):
+        be.activationGrad(np.zeros(16, np.float32), data(be, 16), 4, 4, np.float16, "gelu", out=out)
+    with pytest.raises(ValueError, match="lies on"):
+        be.activationGrad(torch.zeros(16, dtype=torch.float16), data(be, 16), 4, 4, np.float16, "gelu", out=out)
+    with pytest.raises(ValueError, match="type"):
+        be.activationGrad(torch.zeros(16, dtype=torch.bfloat16), data(be, 16), 4, 4, np.float16, "gelu", out=out)
+    with pytest.raises(TypeError, match="device"):
+        be.activationGrad(data(be, 16), data(be, 16), 4, 4, np.float16, "gelu", out=np.zeros(16, np.float16))
+    for dtype in (np.int64, B.DType.int64):
+        with pytest.raises(B.NotImplementedByBackend):
+            be.layerNorm(data(be, 16), None, None, 4, 4, dtype)
+        with pytest.raises(B.NotImplementedByBackend):
+            be.groupedMatmul(1, data(be, 2, 8), data(be, 16), data(be, 16), False, 4, 4, 4, dtype)
+
+
+def test_norm_and_groups_check_sizes(be):
+    stat = lambda n: data(be, n, 4)  # noqa: E731
+    with pytest.raises(ValueError, match="weight is smaller"):
+        be.layerNorm(data(be, 16), stat(3), None, 4, 4, np.float16, out=data(be, 16))
+    with pytest.raises(ValueError, match="mean is smaller"):
+        be.layerNorm(data(be, 16), None, None, 4, 4, np.float16, out=data(be, 16), mean=stat(3))
+    with pytest.raises(ValueError, match="rstd is smaller"):
+        be.layerNormGrad(data(be, 16), data(be, 16), None, stat(4), stat(3), 4, 4, np.float16, out=data(be, 16))
+    with pytest.raises(ValueError, match="offsets is smaller"):
+        be.groupedMatmul(3, data(be, 3, 8), data(be, 16), data(be, 48), False, 4, 4, 4, np.float16, out=data(be, 16))
+    with pytest.raises(ValueError, match="operand b is smaller"):
+        be.groupedMatmul(3, data(be, 4, 8), data(be, 16), data(be, 47), False, 4, 4, 4, np.float16, out=data(be, 16))
+    with pytest.raises(ValueError, match="out is smaller"):
+        be.groupedMatmulWeightGrad(3, data(be, 4, 8), data(be, 16), data(be, 16), 4, 4, 4, np.float16, out=data(be, 47))
+    be.groupedMatmulWeightGrad(3, data(be, 4, 8), data(be, 16), data(be, 16), 4, 4, 4, np.float16, out=data(be, 48), mark=False)
+    assert len(called(be, "hc_grouped_matmul_weight_grad")) == 1
+
+
+def test_adamw_plan(be):
+    row = lambda **k: dict(param=data(be, 8, 4), grad=data(be, 8, 2), moment1=data(be, 8, 4), moment2=data(be, 8, 4), count=8,  # noqa: E731
+                           dtype=np.float32, gradDType=np.float16, **k)
+    plan = be.adamWPlan([row(), row(copy=data(be, 8, 2))])
+    t = plan._table
+    assert plan.count == 2 and t[0].count == 8 and t[0].param_copy is None and t[1].param_copy == 256
+    assert (t[0].param_dtype, t[0].grad_dtype) == (L.HC_F32, L.HC_F16)
+    new = B.CUDAData(be, 512, 16, owns=False)
+    plan.setGrad(1, new)
+    assert t[1].grad == 512
+    with pytest.raises(ValueError, match="smaller"):
+        plan.setGrad(0, data(be, 7, 2))
+    be.adamW(plan, 3, mark=False)
+    (args,) = called(be, "hc_adamw")
+    assert args[2:4] == (2, 3)
+    with pytest.raises(ValueError, match="unknown entries"):
+        be.adamWPlan([row(momentum=None)])
+    with pytest.raises(ValueError, match="dtype"):
+        be.adamWPlan([{k: v for k, v in row().items() if k not in ("dtype", "gradDType")}])
+    with pytest.raises(ValueError, match="copy"):
+        be.adamWPlan([row(copy=data(be, 7, 2))])
