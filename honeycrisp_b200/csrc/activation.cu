@@ -26,26 +26,41 @@ __global__ void __launch_bounds__(kLanes * kWarps) activation_grad_kernel(const 
   float sum[kW];
 #pragma unroll
   for (int e = 0; e < kW; e++) sum[e] = 0.0f;
-  if (col < cols) {
-#pragma unroll 4
-    for (int64_t r = row0 + warp; r < row1; r += kWarps) {
-      const int64_t at = r * cols + col;
-      float x[kW], z[kW];
-      if constexpr (kW == 1) {
-        x[0] = widen_f<T>(grad[at]);
-        z[0] = widen_f<T>(pre[at]);
-      } else {
-        const uint4 gu = *(const uint4*)(grad + at), zu = *(const uint4*)(pre + at);
-        Pack16<T>::widen(gu, x);
-        Pack16<T>::widen(zu, z);
-      }
-      act_scale_t<kAct, sizeof(T) == 2, kW>(x, z);
-      if (kSum)
-#pragma unroll
-        for (int e = 0; e < kW; e++) sum[e] += x[e];
-      if constexpr (kW == 1) dpre[at] = narrow_f<T>(x[0]);
-      else *(uint4*)(dpre + at) = Pack16<T>::narrow(x);
+  // kAhead rows of both inputs are on their way before the first is used (dpre may be one of the inputs, so the compiler cannot move
+  // a load across a store by itself).
+  constexpr int kAhead = kW == 1 ? 8 : 4;
+  typedef typename std::conditional<kW == 1, T, uint4>::type Raw;
+  auto use = [&](int64_t r, const Raw& graw, const Raw& zraw) {
+    float x[kW], z[kW];
+    if constexpr (kW == 1) {
+      x[0] = widen_f<T>(graw);
+      z[0] = widen_f<T>(zraw);
+    } else {
+      Pack16<T>::widen(graw, x);
+      Pack16<T>::widen(zraw, z);
     }
+    act_scale_t<kAct, sizeof(T) == 2, kW>(x, z);
+    if (kSum)
+#pragma unroll
+      for (int e = 0; e < kW; e++) sum[e] += x[e];
+    if constexpr (kW == 1) dpre[r * cols + col] = narrow_f<T>(x[0]);
+    else *(uint4*)(dpre + r * cols + col) = Pack16<T>::narrow(x);
+  };
+  if (col < cols) {
+    int64_t r0 = row0 + warp;
+    for (; r0 + (kAhead - 1) * kWarps < row1; r0 += kAhead * kWarps) {
+      Raw graw[kAhead], zraw[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; i++) {
+        graw[i] = *(const Raw*)(grad + (r0 + i * kWarps) * cols + col);
+        zraw[i] = *(const Raw*)(pre + (r0 + i * kWarps) * cols + col);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; i++) use(r0 + i * kWarps, graw[i], zraw[i]);
+    }
+    // the last rows one by one, in code of their own: a short input runs only these few instructions
+#pragma unroll 1
+    for (; r0 < row1; r0 += kWarps) use(r0, *(const Raw*)(grad + r0 * cols + col), *(const Raw*)(pre + r0 * cols + col));
   }
   if (kSum) {
     __shared__ float tile[kWarps][kLanes * kW];
@@ -90,11 +105,13 @@ __global__ void __launch_bounds__(256) sum_runs_kernel(const float* partial, int
 }  // namespace
 
 RunSplit split_runs(int64_t rows, int64_t cols, int cols_per_cta) {
-  // About eight CTAs for each of 148 SMs, runs of at least 16 rows (two for every warp), and at most 65535 of them.
+  // About eight CTAs for each of 148 SMs, runs of at least 16 rows (two for every warp); up to 64 rows are one run, whose sums
+  // need no second kernel.
   RunSplit s;
   s.strips = (cols + cols_per_cta - 1) / cols_per_cta;
   int64_t runs = (148 * 8 + s.strips - 1) / s.strips;
   if (runs > (rows + 15) / 16) runs = (rows + 15) / 16;
+  if (rows <= 64) runs = 1;
   if (runs < 1) runs = 1;
   s.rows_per_run = (rows + runs - 1) / runs;
   s.rows_per_run = (s.rows_per_run + 7) / 8 * 8;
@@ -131,7 +148,7 @@ cudaError_t launch_typed(const void* grad, const void* pre, int64_t rows, int64_
   int64_t per = s.rows_per_run;
   void* args[] = {(void*)&grad, (void*)&pre, (void*)&dpre, (void*)&partial, (void*)&rows, (void*)&cols, (void*)&per};
   cudaError_t e = launch_behind(fn, args, dim3((unsigned)s.strips, (unsigned)s.runs), dim3(kLanes * kWarps), 0, stream);
-  if (e != cudaSuccess || !bias_grad) return e;
+  if (e != cudaSuccess || !bias_grad || s.runs == 1) return e;   // one run's partial matrix is the sum
   return launch_sum_runs(partial, s.runs, cols, bias_grad, nullptr, false, stream);
 }
 bool rows_of_16_bytes(const void* a, const void* b, const void* c, int64_t row_bytes) {
@@ -151,6 +168,7 @@ cudaError_t launch_activation_grad(hc_dtype dtype, int act, const void* grad, co
   const bool vec = rows_of_16_bytes(grad, pre, dpre, cols * eb);
   const RunSplit s = split_runs(rows, cols, kLanes * (vec ? (int)(16 / eb) : 1));
   if (s.strips > 2147483647LL || s.runs > 65535) return cudaErrorInvalidValue;
+  if (s.runs == 1) scratch = bias_grad;
   return dtype == HC_F16 ? launch_typed<__half>(grad, pre, rows, cols, dpre, bias_grad, scratch, vec, s, act, stream)
                          : launch_typed<float>(grad, pre, rows, cols, dpre, bias_grad, scratch, vec, s, act, stream);
 }

@@ -1319,6 +1319,33 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
               bulk_commit();
             }
           }
+        } else if constexpr (kMode == kGrouped) {
+          // A warp at a group's end, or a result TMA cannot describe: through the staging buffer all the same, then a row
+          // at a time by the whole warp (a row a lane would touch 32 sectors for every few bytes).
+          const int rows_here = (int)min((int64_t)32, row_end - (gm - lane));
+          if (store_leader) bulk_wait_read<0>();
+          __syncwarp();
+          const uint32_t own_row = stg_base + (uint32_t)lane * 128u, sw = (uint32_t)(lane & 7);
+#pragma unroll 1
+          for (int c = 0; rows_here > 0 && c < COLS_PER_PART && n0h + c < p.N; c += 64) {
+#pragma unroll
+            for (int l = 0; l < 2; l++) {
+              uint32_t r[32];
+              tmem_ld_x32(tbase + c + 32 * l, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int q = 0; q < 4; q++) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = __uint_as_float(r[q * 8 + e]);
+                const uint4 u = Pack16<__half>::narrow(x);
+                st_shared_v4(own_row + (((uint32_t)(q + 4 * l) ^ sw) << 4), u.x, u.y, u.z, u.w);
+              }
+            }
+            __syncwarp();
+            block_to_memory<__half>(stg_base, (__half*)cmat + (gm - lane) * p.ldc + n0h + c, p.ldc, rows_here, (int)min((int64_t)64, p.N - n0h - c));
+            __syncwarp();
+          }
         } else {
 #pragma unroll 1
           for (int c = 0; c < COLS_PER_PART; c += 32) {
@@ -1454,6 +1481,22 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
               for (int d = 0; d < p.n_out; d++) tma_store_3d(&mapC.m[d], stg_base, (int)(n0 + c), m_warp, (int)t.mat);
               bulk_commit();
             }
+          }
+        } else if constexpr (kMode == kGrouped) {
+          const int rows_here = (int)min((int64_t)32, row_end - (gm - lane));
+          if (store_leader) bulk_wait_read<0>();
+          __syncwarp();
+          const uint32_t own_row = stg_base + (uint32_t)lane * 128u, sw = (uint32_t)(lane & 7);
+#pragma unroll
+          for (int c = 0; c < COLS_PER_THREAD; c += 32) {
+            if (!ok || rows_here <= 0 || n0 + c >= p.N) continue;
+#pragma unroll
+            for (int q = 0; q < 8; q++)
+              st_shared_v4(own_row + (((uint32_t)q ^ sw) << 4), __float_as_uint(acc[c + q * 4]), __float_as_uint(acc[c + q * 4 + 1]),
+                           __float_as_uint(acc[c + q * 4 + 2]), __float_as_uint(acc[c + q * 4 + 3]));
+            __syncwarp();
+            block_to_memory<float>(stg_base, (float*)cmat + (gm - lane) * p.ldc + n0 + c, p.ldc, rows_here, (int)min((int64_t)32, p.N - n0 - c));
+            __syncwarp();
           }
         } else if (ok && gm < row_end) {
 #pragma unroll
