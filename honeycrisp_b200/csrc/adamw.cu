@@ -18,7 +18,7 @@ namespace {
 
 constexpr int kMaxTensors = 448;          // 448 x 56 bytes: below the 32764 bytes of kernel parameters
 constexpr int kThreads = 256;
-constexpr int kQuads = 4;                 // groups of four elements a thread updates
+constexpr int kQuads = 2;                 // groups of four elements a thread updates
 constexpr int kChunk = kThreads * kQuads * 4;
 
 struct AdamTensor {
@@ -67,10 +67,10 @@ __device__ __forceinline__ float4 load_four(const void* p, int half, int64_t k) 
 }
 __device__ __forceinline__ void store_four(void* p, int half, int64_t k, const float4& x) {
   if (!half) {
-    *(float4*)((float*)p + k) = x;
+    __stcs((float4*)((float*)p + k), x);
   } else {
     const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
-    *(uint2*)((__half*)p + k) = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
+    __stcs((uint2*)((__half*)p + k), make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b));
   }
 }
 

@@ -13,6 +13,26 @@
 namespace hc {
 namespace {
 
+// Two float32 operations in one instruction; each lane rounds as its scalar form does.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(*(unsigned long long*)&r)
+      : "l"(*(const unsigned long long*)&a), "l"(*(const unsigned long long*)&b), "l"(*(const unsigned long long*)&c));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(*(unsigned long long*)&r) : "l"(*(const unsigned long long*)&a), "l"(*(const unsigned long long*)&b));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(*(unsigned long long*)&r) : "l"(*(const unsigned long long*)&a), "l"(*(const unsigned long long*)&b));
+  return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 struct NormJob {
   const void* x;
   const void* grad;     // backward
@@ -327,22 +347,36 @@ __global__ void __launch_bounds__(kThreads* kRows, kThreads * kRows <= 256 ? 2 :
     }
   };
   statistics(row);
-  float w[E], dw[E], db[E];
-  load_params<kW, kC, kThreads>(j.w, j.param_half, 1.0f, j.cols, t, w);
+  // Elements in pairs: the pass is bound by instructions as much as by memory, and a pair costs one of each kind.
+  constexpr int P = E / 2;
+  float2 w[P], dw[P], db[P];
+  {
+    float all[E];
+    load_params<kW, kC, kThreads>(j.w, j.param_half, 1.0f, j.cols, t, all);
 #pragma unroll
-  for (int e = 0; e < E; e++) dw[e] = db[e] = 0.0f;
+    for (int e = 0; e < P; e++) {
+      w[e] = make_float2(all[2 * e], all[2 * e + 1]);
+      dw[e] = db[e] = make_float2(0.0f, 0.0f);
+    }
+  }
   int slot = 0;
   uint32_t at = 0;
   for (; row < rows; row += stride, src_x += step, src_g += step, dst += step) {
-    float h[kBatch][E], g[kBatch][E];
+    float2 h[kBatch][P], g[kBatch][P];
     if constexpr (Q::kAsync) {
       fetch((D - 1) * step, row + (D - 1) * stride, at == 0 ? D - 1 : at - 1);
       queue_wait<D - 1>();
     }
 #pragma unroll
     for (int r = 0; r < kBatch; r++) {
-      qx.take(r, at, row + r < rows, h[r]);
-      qg.take(r, at, row + r < rows, g[r]);
+      float xv[E], gv[E];
+      qx.take(r, at, row + r < rows, xv);
+      qg.take(r, at, row + r < rows, gv);
+#pragma unroll
+      for (int e = 0; e < P; e++) {
+        h[r][e] = make_float2(xv[2 * e], xv[2 * e + 1]);
+        g[r][e] = make_float2(gv[2 * e], gv[2 * e + 1]);
+      }
     }
     at = at + 1 == D ? 0 : at + 1;
     if constexpr (!Q::kAsync) fetch(step, row + stride, 0);
@@ -350,17 +384,19 @@ __global__ void __launch_bounds__(kThreads* kRows, kThreads * kRows <= 256 ? 2 :
 #pragma unroll
     for (int r = 0; r < kBatch; r++) {
       rstd[r] = rstd_at[r];
-      const float off = -mean_at[r] * rstd[r];
-      s[2 * r] = s[2 * r + 1] = 0.0f;
+      const float2 scale = both(rstd[r]), off = both(-mean_at[r] * rstd[r]);
+      float2 s0 = both(0.0f), s1 = both(0.0f);
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        h[r][e] = fmaf(h[r][e], rstd[r], off);   // past the row's end g is zero, and so is all that follows from it
-        db[e] += g[r][e];
-        dw[e] = fmaf(g[r][e], h[r][e], dw[e]);
-        g[r][e] *= w[e];
-        s[2 * r] += g[r][e];
-        s[2 * r + 1] = fmaf(g[r][e], h[r][e], s[2 * r + 1]);
+      for (int e = 0; e < P; e++) {
+        h[r][e] = fma2(h[r][e], scale, off);   // past the row's end g is zero, and so is all that follows from it
+        db[e] = add2(db[e], g[r][e]);
+        dw[e] = fma2(g[r][e], h[r][e], dw[e]);
+        g[r][e] = mul2(g[r][e], w[e]);
+        s0 = add2(s0, g[r][e]);
+        s1 = fma2(g[r][e], h[r][e], s1);
       }
+      s[2 * r] = s0.x + s0.y;
+      s[2 * r + 1] = s1.x + s1.y;
     }
     statistics(row + stride);
     row_sum<kThreads, kRows, 2 * kBatch>(s, scratch, slot);
@@ -368,14 +404,20 @@ __global__ void __launch_bounds__(kThreads* kRows, kThreads * kRows <= 256 ? 2 :
 #pragma unroll
       for (int r = 0; r < kBatch; r++) {
         if (row + r >= rows) continue;
-        const float m0 = -s[2 * r] * inv_n, m1 = -s[2 * r + 1] * inv_n;
+        const float2 scale = both(rstd[r]), m0 = both(-s[2 * r] * inv_n), m1 = both(-s[2 * r + 1] * inv_n);
+        float out[E];
 #pragma unroll
-        for (int e = 0; e < E; e++) g[r][e] = rstd[r] * fmaf(h[r][e], m1, g[r][e] + m0);
-        qx.store(dst + r * j.cols, g[r]);
+        for (int e = 0; e < P; e++) {
+          const float2 v = mul2(scale, fma2(h[r][e], m1, add2(g[r][e], m0)));
+          out[2 * e] = v.x;
+          out[2 * e + 1] = v.y;
+        }
+        qx.store(dst + r * j.cols, out);
       }
     }
   }
   if (!partial) return;
+  auto of = [](const float2 (&v)[P], int e) { return e & 1 ? v[e / 2].y : v[e / 2].x; };
   float* to[2] = {partial + (int64_t)blockIdx.x * j.cols, partial + ((int64_t)gridDim.x + blockIdx.x) * j.cols};
   if (kRows == 1) {
 #pragma unroll
@@ -383,7 +425,7 @@ __global__ void __launch_bounds__(kThreads* kRows, kThreads * kRows <= 256 ? 2 :
 #pragma unroll
       for (int e = 0; e < kW; e++) {
         const int64_t k = (int64_t)(t + c * kThreads) * kW + e;
-        if (k < j.cols) { to[0][k] = dw[c * kW + e]; to[1][k] = db[c * kW + e]; }
+        if (k < j.cols) { to[0][k] = of(dw, c * kW + e); to[1][k] = of(db, c * kW + e); }
       }
   } else {
     constexpr int N = kThreads * E;
@@ -395,8 +437,8 @@ __global__ void __launch_bounds__(kThreads* kRows, kThreads * kRows <= 256 ? 2 :
 #pragma unroll
       for (int e = 0; e < kW; e++) {
         const int k = (t + c * kThreads) * kW + e;
-        columns[sub * N + k] = dw[c * kW + e];
-        columns[(kRows + sub) * N + k] = db[c * kW + e];
+        columns[sub * N + k] = of(dw, c * kW + e);
+        columns[(kRows + sub) * N + k] = of(db, c * kW + e);
       }
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * N; i += kThreads * kRows) {
