@@ -287,6 +287,25 @@ class AdamWPlan:
                     self._updated.append(x)
             row.count = count
             row.param_dtype, row.grad_dtype = _HC_DTYPE[pd], _HC_DTYPE[gd]
+        self._refuse_overlaps()
+
+    def _refuse_overlaps(self) -> None:
+        """One launch updates all tensors at once: nothing it writes may be another tensor's (a parameter that is listed
+        twice, as tied weights are, would be updated twice at the same time)."""
+        spans = []
+        for i, r in enumerate(self._table[: self.count]):
+            pb, gb = (2 if t == L.HC_F16 else 4 for t in (r.param_dtype, r.grad_dtype))
+            for name, start, size, written in (("param", r.param, pb, True), ("moment1", r.moment1, 4, True), ("moment2", r.moment2, 4, True),
+                                               ("copy", r.param_copy, 2, True), ("grad", r.grad, gb, False)):
+                if start and r.count:
+                    spans.append((start, start + r.count * size, written, f"{name} of tensor {i}"))
+        reach, last = {True: 0, False: 0}, {True: "", False: ""}
+        for start, end, written, name in sorted(spans):
+            for other in ((True, False) if written else (True,)):
+                if start < reach[other]:
+                    raise ValueError(f"AdamWPlan: {name} overlaps {last[other]}")
+            if end > reach[written]:
+                reach[written], last[written] = end, name
 
     def setGrad(self, index: int, grad) -> None:
         """Tensor `index` takes its gradient from `grad` (of the same type and length) from now on."""

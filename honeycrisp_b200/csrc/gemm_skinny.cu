@@ -263,7 +263,7 @@ SkinnyPlan plan_skinny(const GemmProblem& p, int sm_count) {
 }  // namespace
 
 bool skinny_fits(const GemmProblem& p) {
-  return p.fused && p.batch == 1 && p.M >= 1 && p.M <= 8 && !p.a_mn_major && p.K >= 1 && p.K < (1ll << 26) && p.N < (1ll << 31) - 1024;
+  return p.fused && p.batch == 1 && p.M >= 1 && p.M <= 8 && !p.a_mn_major && p.K >= 1 && p.K < (1ll << 25) && p.N < (1ll << 31) - 1024;
 }
 
 bool skinny_preferred(const GemmProblem& p) {

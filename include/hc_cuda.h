@@ -18,6 +18,9 @@
  * Pointers are device pointers on the context's device unless a function says "host".
  * Work is enqueued on the context's stream and the call returns without waiting; inputs must
  * stay alive until the stream has passed the call (hc_sync / hc_event_wait).
+ * Products that need a work area share the context's: what one context enqueues, captured graphs included, runs in the
+ * order of one stream (use a context for each stream that is to overlap another).  A graph keeps the work area of its
+ * capture valid until hc_destroy; replay none after it.
  * All functions are thread-safe; calls on one context are ordered by a mutex, which is the
  * same discipline as the reference backends' single worker thread
  * (Sources/Honeycrisp/BackendCPU.swift:235-248).

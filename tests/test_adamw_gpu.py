@@ -124,7 +124,10 @@ def test_refusals(be):
         with pytest.raises(ValueError, match=what):
             be.adamW(plan, **bad)
     with pytest.raises(ValueError, match="overlap"):
-        be.adamW(be.adamWPlan([dict(param=t[0], grad=t[1], moment1=t[2], moment2=t[2])]), 1)
+        be.adamWPlan([dict(param=t[0], grad=t[1], moment1=t[2], moment2=t[2])])
+    plan._table[0].moment2 = plan._table[0].moment1          # past the plan's own check, the library's
+    with pytest.raises(ValueError, match="overlap"):
+        be.adamW(plan, 1)
     with pytest.raises(ValueError, match="smaller"):
         be.adamWPlan([dict(param=t[0], grad=t[1][:5], moment1=t[2], moment2=t[3])])
     with pytest.raises(ValueError, match="type"):

@@ -92,6 +92,41 @@ def test_cut_contractions(diag, monkeypatch, dtype):
             forward_case(diag, rows, inner, cols, dtype, "gelu", True, True, True)
 
 
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("tb", [False, True])
+def test_few_columns_and_long_contractions(be, dtype, tb):
+    """A result of one to three columns over a long contraction: one tile, cut into parts."""
+    for rows, inner, cols in [(9, 256, 1), (16, 300, 3), (40, 2048, 2), (8, 1500, 1), (1, 40000, 5), (7, 1030, 640)]:
+        forward_case(be, rows, inner, cols, dtype, "silu", True, True, False, tb=tb)
+
+
+def test_two_contexts_at_once(be):
+    """Two contexts on two streams, the same inputs, calls enqueued in turn: each has its own work area."""
+    import torch
+    from honeycrisp_b200 import CUDABackend
+    rng = np.random.default_rng(1)
+    rows, inner, cols = 4, 4096, 1000                     # partial sums in the work area
+    a, b, _, _ = operands(rng, rows, inner, cols, np.float16)
+    ad, bd = torch.from_numpy(a).cuda(), torch.from_numpy(b).cuda()
+    others = [CUDABackend(0) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in others]
+    outs = [torch.empty(8, rows, cols, dtype=torch.float16, device="cuda") for _ in others]
+    torch.cuda.synchronize()
+    for o, s in zip(others, streams):
+        o.useStream(s.cuda_stream)
+    for i in range(8):
+        for o, out in zip(others, outs):
+            o.matmulEpilogue(ad, False, bd, False, rows, inner, cols, np.float16, activation="gelu" if i % 2 else "relu", out=out[i], mark=False)
+    torch.cuda.synchronize()
+    for i in range(8):
+        want = be.matmulEpilogue(a, False, b, False, rows, inner, cols, np.float16, activation="gelu" if i % 2 else "relu").onCPU(np.float16)
+        for out in outs:
+            assert np.array_equal(out[i].cpu().numpy().reshape(-1), want[: rows * cols])
+    for o in others:
+        o.checkDeviceStatus()
+        o.close()
+
+
 def test_empty_sizes(be):
     """An empty contraction leaves bias, activation and residual; no rows or no columns leave nothing to do."""
     forward_case(be, 5, 0, 9, np.float16, "silu", True, True, True)

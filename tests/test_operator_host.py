@@ -108,17 +108,20 @@ def test_norm_and_groups_check_sizes(be):
 
 
 def test_adamw_plan(be):
-    row = lambda **k: dict(param=data(be, 8, 4), grad=data(be, 8, 2), moment1=data(be, 8, 4), moment2=data(be, 8, 4), count=8,  # noqa: E731
+    at = iter(range(1 << 10, 1 << 30, 256))
+    new = lambda n, size: B.CUDAData(be, next(at), n * size, owns=False)  # noqa: E731
+    row = lambda **k: dict(param=new(8, 4), grad=new(8, 2), moment1=new(8, 4), moment2=new(8, 4), count=8,  # noqa: E731
                            dtype=np.float32, gradDType=np.float16, **k)
-    plan = be.adamWPlan([row(), row(copy=data(be, 8, 2))])
+    copy = new(8, 2)
+    plan = be.adamWPlan([row(), row(copy=copy)])
     t = plan._table
-    assert plan.count == 2 and t[0].count == 8 and t[0].param_copy is None and t[1].param_copy == 256
+    assert plan.count == 2 and t[0].count == 8 and t[0].param_copy is None and t[1].param_copy == copy.ptr
     assert (t[0].param_dtype, t[0].grad_dtype) == (L.HC_F32, L.HC_F16)
-    new = B.CUDAData(be, 512, 16, owns=False)
-    plan.setGrad(1, new)
-    assert t[1].grad == 512
+    grad = new(8, 2)
+    plan.setGrad(1, grad)
+    assert t[1].grad == grad.ptr
     with pytest.raises(ValueError, match="smaller"):
-        plan.setGrad(0, data(be, 7, 2))
+        plan.setGrad(0, new(7, 2))
     be.adamW(plan, 3, mark=False)
     (args,) = called(be, "hc_adamw")
     assert args[2:4] == (2, 3)
@@ -127,4 +130,19 @@ def test_adamw_plan(be):
     with pytest.raises(ValueError, match="dtype"):
         be.adamWPlan([{k: v for k, v in row().items() if k not in ("dtype", "gradDType")}])
     with pytest.raises(ValueError, match="copy"):
-        be.adamWPlan([row(copy=data(be, 7, 2))])
+        be.adamWPlan([row(copy=new(7, 2))])
+
+
+def test_adamw_plan_refuses_what_two_tensors_share(be):
+    at = iter(range(1 << 10, 1 << 30, 256))
+    new = lambda: B.CUDAData(be, next(at), 32, owns=False)  # noqa: E731
+    row = lambda **k: dict(dict(param=new(), grad=new(), moment1=new(), moment2=new(), count=8, dtype=np.float32), **k)  # noqa: E731
+    tied, grad = new(), new()
+    with pytest.raises(ValueError, match="param of tensor 1 overlaps param of tensor 0"):
+        be.adamWPlan([row(param=tied), row(param=tied)])
+    with pytest.raises(ValueError, match="overlaps"):
+        be.adamWPlan([row(), row(grad=tied), row(moment2=tied)])
+    with pytest.raises(ValueError, match="overlaps"):
+        be.adamWPlan([row(param=B.CUDAData(be, 1 << 9, 32, owns=False)), row(moment1=B.CUDAData(be, (1 << 9) + 28, 32, owns=False))])
+    be.adamWPlan([row(grad=grad), row(grad=grad)])       # a gradient is only read
+    be.adamWPlan([row(param=B.CUDAData(be, 1 << 9, 32, owns=False)), row(param=B.CUDAData(be, (1 << 9) + 32, 32, owns=False))])
