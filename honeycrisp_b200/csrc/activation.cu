@@ -26,41 +26,67 @@ __global__ void __launch_bounds__(kLanes * kWarps) activation_grad_kernel(const 
   float sum[kW];
 #pragma unroll
   for (int e = 0; e < kW; e++) sum[e] = 0.0f;
-  // kAhead rows of both inputs are on their way before the first is used (dpre may be one of the inputs, so the compiler cannot move
-  // a load across a store by itself).
-  constexpr int kAhead = kW == 1 ? 8 : 4;
-  typedef typename std::conditional<kW == 1, T, uint4>::type Raw;
-  auto use = [&](int64_t r, const Raw& graw, const Raw& zraw) {
-    float x[kW], z[kW];
-    if constexpr (kW == 1) {
-      x[0] = widen_f<T>(graw);
-      z[0] = widen_f<T>(zraw);
-    } else {
-      Pack16<T>::widen(graw, x);
-      Pack16<T>::widen(zraw, z);
-    }
+  auto use = [&](int64_t at, float (&x)[kW], const float (&z)[kW]) {
     act_scale_t<kAct, sizeof(T) == 2, kW>(x, z);
     if (kSum)
 #pragma unroll
       for (int e = 0; e < kW; e++) sum[e] += x[e];
-    if constexpr (kW == 1) dpre[r * cols + col] = narrow_f<T>(x[0]);
-    else *(uint4*)(dpre + r * cols + col) = Pack16<T>::narrow(x);
+    if constexpr (kW == 1) dpre[at] = narrow_f<T>(x[0]);
+    else *(uint4*)(dpre + at) = Pack16<T>::narrow(x);
   };
-  if (col < cols) {
+  // Rows of both inputs travel ahead of their use (dpre may be one of the inputs, so the compiler cannot move a load across a
+  // store by itself; a thread's rows ahead are its own and still unwritten).  16-byte chunks wait in shared memory, where each
+  // thread reads back what it copied itself, three rows ahead; single elements in registers, eight rows at a time.
+  if constexpr (kW > 1) {
+    constexpr int kDepth = 4;
+    __shared__ uint4 queue[kDepth][2][kLanes * kWarps];
+    if (col < cols) {
+      const int64_t step = kWarps * cols;
+      const int mine = (int)((row1 - row0 - warp + kWarps - 1) / kWarps);   // rows of this warp (negative: none)
+      const T *g_at = grad + (row0 + warp) * cols + col, *z_at = pre + (row0 + warp) * cols + col;
+      auto fetch = [&](int i) {
+        if (i < mine) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&queue[i % kDepth][0][threadIdx.x])), "l"(g_at + i * step) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&queue[i % kDepth][1][threadIdx.x])), "l"(z_at + i * step) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+#pragma unroll
+      for (int i = 0; i < kDepth - 1; i++) fetch(i);
+#pragma unroll 1
+      for (int i = 0; i < mine; i++) {
+        fetch(i + kDepth - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+        float x[kW], z[kW];
+        Pack16<T>::widen(queue[i % kDepth][0][threadIdx.x], x);
+        Pack16<T>::widen(queue[i % kDepth][1][threadIdx.x], z);
+        use((row0 + warp + (int64_t)i * kWarps) * cols + col, x, z);
+      }
+    }
+  } else if (col < cols) {
+    constexpr int kAhead = 8;
     int64_t r0 = row0 + warp;
     for (; r0 + (kAhead - 1) * kWarps < row1; r0 += kAhead * kWarps) {
-      Raw graw[kAhead], zraw[kAhead];
+      T graw[kAhead], zraw[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; i++) {
-        graw[i] = *(const Raw*)(grad + (r0 + i * kWarps) * cols + col);
-        zraw[i] = *(const Raw*)(pre + (r0 + i * kWarps) * cols + col);
+        graw[i] = grad[(r0 + i * kWarps) * cols + col];
+        zraw[i] = pre[(r0 + i * kWarps) * cols + col];
       }
 #pragma unroll
-      for (int i = 0; i < kAhead; i++) use(r0 + i * kWarps, graw[i], zraw[i]);
+      for (int i = 0; i < kAhead; i++) {
+        float x[1] = {widen_f<T>(graw[i])};
+        const float z[1] = {widen_f<T>(zraw[i])};
+        use((r0 + i * kWarps) * cols + col, x, z);
+      }
     }
     // the last rows one by one, in code of their own: a short input runs only these few instructions
 #pragma unroll 1
-    for (; r0 < row1; r0 += kWarps) use(r0, *(const Raw*)(grad + r0 * cols + col), *(const Raw*)(pre + r0 * cols + col));
+    for (; r0 < row1; r0 += kWarps) {
+      float x[1] = {widen_f<T>(grad[r0 * cols + col])};
+      const float z[1] = {widen_f<T>(pre[r0 * cols + col])};
+      use(r0 * cols + col, x, z);
+    }
   }
   if (kSum) {
     __shared__ float tile[kWarps][kLanes * kW];
@@ -78,10 +104,11 @@ __global__ void __launch_bounds__(kLanes * kWarps) activation_grad_kernel(const 
   }
 }
 
-// out[c] = sum over runs of partial[run][c], for one or two stacks of partial matrices: 32 columns a CTA, every warp
-// sums each eighth run, the eight sums are added in order.
-__global__ void __launch_bounds__(256) sum_runs_kernel(const float* partial, int64_t runs, int64_t cols, void* out0, void* out1,
-                                                       int half) {
+// out[c] = sum over runs of partial[run][c], for one or two stacks of partial matrices: 32 columns a CTA, each of 32 warps sums every
+// 32nd run, the 32 sums are added in order.
+constexpr int kSumWarps = 32;
+__global__ void __launch_bounds__(32 * kSumWarps) sum_runs_kernel(const float* partial, int64_t runs, int64_t cols, void* out0, void* out1,
+                                                                  int half) {
   pdl_wait();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
@@ -90,13 +117,13 @@ __global__ void __launch_bounds__(256) sum_runs_kernel(const float* partial, int
   float s = 0.0f;
   if (c < cols)
 #pragma unroll 8
-    for (int64_t r = warp; r < runs; r += 8) s += src[r * cols + c];
-  __shared__ float tile[8][33];
+    for (int64_t r = warp; r < runs; r += kSumWarps) s += src[r * cols + c];
+  __shared__ float tile[kSumWarps][33];
   tile[warp][lane] = s;
   __syncthreads();
   if (warp == 0 && c < cols && out) {
 #pragma unroll
-    for (int w = 1; w < 8; w++) s += tile[w][lane];
+    for (int w = 1; w < kSumWarps; w++) s += tile[w][lane];
     if (half) ((__half*)out)[c] = __float2half_rn(s);
     else ((float*)out)[c] = s;
   }
@@ -124,7 +151,8 @@ RunSplit split_runs(int64_t rows, int64_t cols, int cols_per_cta) {
 cudaError_t launch_sum_runs(const float* partial, int64_t runs, int64_t cols, void* out0, void* out1, bool half, cudaStream_t stream) {
   int h = half ? 1 : 0;
   void* args[] = {(void*)&partial, (void*)&runs, (void*)&cols, (void*)&out0, (void*)&out1, (void*)&h};
-  return launch_behind((const void*)sum_runs_kernel, args, dim3((unsigned)((cols + 31) / 32), out1 ? 2 : 1), dim3(256), 0, stream);
+  return launch_behind((const void*)sum_runs_kernel, args, dim3((unsigned)((cols + 31) / 32), out1 ? 2 : 1), dim3(32 * kSumWarps), 0,
+                       stream);
 }
 
 namespace {

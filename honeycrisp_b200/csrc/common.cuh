@@ -129,6 +129,12 @@ struct GroupedProblem {
   const void *a, *b;
   void* out;
 };
+// The groups' rows and the tiles in front of each group, as group_setup_kernel lays them out on the device.
+struct GroupTiles { const int *start, *end, *first_tile; int groups; };
+// Groups of few rows on the CUDA cores (csrc/gemm_skinny.cu): tiles of eight rows by a strip of few_strips() a matrix.
+bool few_preferred(const GroupedProblem& p);
+int few_strips(const GroupedProblem& p);
+cudaError_t launch_few(const GroupedProblem& p, const GroupTiles& t, int64_t tiles, cudaStream_t stream);
 cudaError_t launch_grouped(const GroupedProblem& p, cudaStream_t stream, unsigned int* status_word, void* scratch,
                            size_t scratch_bytes, int sm_count, LaunchRecord* rec, size_t* scratch_needed);
 }  // namespace hc

@@ -22,10 +22,9 @@ namespace hc {
 // and the slope is S + z S'.
 //
 // Phi(-y) = e^(-y^2/2) Q(y) for y >= 0 and Phi(y) = 1 - Phi(-y), where Q falls slowly from 1/2 and is fitted
-// by t R(t), t = 1/(1 + p y), R a polynomial, with least largest relative error over y <= 14 (Phi(-14) is
-// 8e-45, below float32's normals): degree 7, p = 0.3, 1.5e-7, for float32 results; degree 5, p = 0.31, 4.7e-6, for float16
-// ones, whose rounding is 4.9e-4.  In float32 the exponent's rounding dominates: 6e-7 of Phi at z = -3,
-// 1.3e-6 at -6.  kFast also takes the hardware's exponential and reciprocal (a few 2^-23).
+// by t R(t), t = 1/(1 + 0.3 y), R a polynomial of degree 7, with least largest relative error over y <= 14 (Phi(-14) is 8e-45,
+// below float32's normals): 1.5e-7.  The exponent's rounding dominates: 6e-7 of Phi at z = -3, 1.3e-6 at -6.
+// kFast, for float16 results, takes the hardware's exponential and reciprocal (a few 2^-23).
 __device__ __forceinline__ float exp2_approx(float t) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
@@ -42,51 +41,90 @@ __device__ __forceinline__ float recip_f(float d) {
   return r;
 }
 
+// Two float32 operations in one instruction; each lane rounds as its scalar form does.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(*(unsigned long long*)&r)
+      : "l"(*(const unsigned long long*)&a), "l"(*(const unsigned long long*)&b), "l"(*(const unsigned long long*)&c));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(*(unsigned long long*)&r) : "l"(*(const unsigned long long*)&a), "l"(*(const unsigned long long*)&b));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(*(unsigned long long*)&r) : "l"(*(const unsigned long long*)&a), "l"(*(const unsigned long long*)&b));
+  return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 constexpr float kTanh1 = 1.5957691216057308f, kTanh3 = kTanh1 * 0.044715f;   // 2 sqrt(2/pi), and times 0.044715
 
 // Phi(z), and e^(-z^2/2) for the slope.
 template <bool kFast>
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
   const float y = fabsf(z);
-  const float t = recip_f<kFast>(fmaf(kFast ? 0.31f : 0.3f, y, 1.0f));
-  float r;
-  if (kFast) {
-    r = -0.07392915338277817f;
-    r = fmaf(r, t, 0.18045039474964142f);
-    r = fmaf(r, t, 0.015744661912322044f);
-    r = fmaf(r, t, 0.13342981040477753f);
-    r = fmaf(r, t, 0.12044127285480499f);
-    r = fmaf(r, t, 0.12386070191860199f);
-  } else {
-    r = 0.035674773156642914f;
-    r = fmaf(r, t, -0.1572030782699585f);
-    r = fmaf(r, t, 0.20635350048542023f);
-    r = fmaf(r, t, -0.05368364229798317f);
-    r = fmaf(r, t, 0.12856163084506989f);
-    r = fmaf(r, t, 0.09991349279880524f);
-    r = fmaf(r, t, 0.12075395882129669f);
-    r = fmaf(r, t, 0.11962930113077164f);
-  }
+  const float t = recip_f<kFast>(fmaf(0.3f, y, 1.0f));
+  float r = 0.035674773156642914f;
+  r = fmaf(r, t, -0.1572030782699585f);
+  r = fmaf(r, t, 0.20635350048542023f);
+  r = fmaf(r, t, -0.05368364229798317f);
+  r = fmaf(r, t, 0.12856163084506989f);
+  r = fmaf(r, t, 0.09991349279880524f);
+  r = fmaf(r, t, 0.12075395882129669f);
+  r = fmaf(r, t, 0.11962930113077164f);
   e = kFast ? exp2_approx(-0.72134752044448170f * y * y) : expf(-0.5f * y * y);
   const float tail = t * r * e;
   return z < 0.0f ? tail : 1.0f - tail;   // NaN: 1 - NaN
 }
 
+// The same for two values, as float16 results take it: 15 instructions a value instead of 26.
+__device__ __forceinline__ float2 normal_cdf_pair(float2 z, float2& e) {
+  const float2 y = make_float2(fabsf(z.x), fabsf(z.y));
+  const float2 d = fma2(both(0.3f), y, both(1.0f));
+  const float2 t = make_float2(recip_f<true>(d.x), recip_f<true>(d.y));
+  float2 r = fma2(both(0.035674773156642914f), t, both(-0.1572030782699585f));
+  r = fma2(r, t, both(0.20635350048542023f));
+  r = fma2(r, t, both(-0.05368364229798317f));
+  r = fma2(r, t, both(0.12856163084506989f));
+  r = fma2(r, t, both(0.09991349279880524f));
+  r = fma2(r, t, both(0.12075395882129669f));
+  r = fma2(r, t, both(0.11962930113077164f));
+  const float2 q = mul2(mul2(y, both(-0.72134752044448170f)), y);
+  e = make_float2(exp2_approx(q.x), exp2_approx(q.y));
+  const float2 tail = mul2(mul2(t, r), e), rest = fma2(both(-1.0f), tail, both(1.0f));
+  return make_float2(z.x < 0.0f ? tail.x : rest.x, z.y < 0.0f ? tail.y : rest.y);
+}
+
 template <int kAct, bool kFast, int W>
 __device__ __forceinline__ void act_apply_t(float (&x)[W]) {
+  if constexpr (kAct == HC_ACT_GELU && kFast && W % 2 == 0) {
 #pragma unroll
-  for (int e = 0; e < W; e++) {
-    const float z = x[e];
-    if (kAct == HC_ACT_RELU) x[e] = z < 0.0f ? 0.0f : z;   // keeps NaN
-    if (kAct == HC_ACT_SILU) x[e] = z * recip_f<kFast>(1.0f + exp_f<kFast>(-1.0f, z));
-    if (kAct == HC_ACT_GELU_TANH) {
-      const float q = kFast ? exp2_approx(z * fmaf(-1.4426950408889634f * kTanh3 * z, z, -1.4426950408889634f * kTanh1))
-                            : expf(-z * fmaf(kTanh3 * z, z, kTanh1));
-      x[e] = z * recip_f<kFast>(1.0f + q);
+    for (int e = 0; e < W; e += 2) {
+      const float2 z = make_float2(x[e], x[e + 1]);
+      float2 g;
+      const float2 v = mul2(z, normal_cdf_pair(z, g));
+      x[e] = v.x;
+      x[e + 1] = v.y;
     }
-    if (kAct == HC_ACT_GELU) {
-      float g;
-      x[e] = z * normal_cdf<kFast>(z, g);
+  } else {
+#pragma unroll
+    for (int e = 0; e < W; e++) {
+      const float z = x[e];
+      if (kAct == HC_ACT_RELU) x[e] = z < 0.0f ? 0.0f : z;   // keeps NaN
+      if (kAct == HC_ACT_SILU) x[e] = z * recip_f<kFast>(1.0f + exp_f<kFast>(-1.0f, z));
+      if (kAct == HC_ACT_GELU_TANH) {
+        const float q = kFast ? exp2_approx(z * fmaf(-1.4426950408889634f * kTanh3 * z, z, -1.4426950408889634f * kTanh1))
+                              : expf(-z * fmaf(kTanh3 * z, z, kTanh1));
+        x[e] = z * recip_f<kFast>(1.0f + q);
+      }
+      if (kAct == HC_ACT_GELU) {
+        float g;
+        x[e] = z * normal_cdf<kFast>(z, g);
+      }
     }
   }
 }
@@ -95,22 +133,35 @@ __device__ __forceinline__ void act_apply_t(float (&x)[W]) {
 // not arise: beyond |z| = 16 (SILU 80) the slope is 0 or 1 to float32, so z is bounded there first.
 template <int kAct, bool kFast, int W>
 __device__ __forceinline__ void act_scale_t(float (&x)[W], const float (&pre)[W]) {
-  constexpr float kBound = kAct == HC_ACT_SILU ? 80.0f : 16.0f;
-  constexpr float k1 = kAct == HC_ACT_SILU ? 1.0f : kTanh1, k3 = kAct == HC_ACT_SILU ? 0.0f : kTanh3;
+  if constexpr (kAct == HC_ACT_GELU && kFast && W % 2 == 0) {
 #pragma unroll
-  for (int e = 0; e < W; e++) {
-    if (kAct == HC_ACT_RELU) x[e] = pre[e] <= 0.0f ? 0.0f : x[e];
-    const float z = pre[e] != pre[e] ? pre[e] : fminf(fmaxf(pre[e], -kBound), kBound);
-    if (kAct == HC_ACT_SILU || kAct == HC_ACT_GELU_TANH) {
-      const float q = exp_f<kFast>(-1.0f, fabsf(z) * fmaf(k3 * z, z, k1));   // in (0, 1]: both sigmas from it
-      const float d = recip_f<kFast>(1.0f + q);
-      const float s = z < 0.0f ? q * d : d;
-      x[e] *= fmaf(z * fmaf(3.0f * k3 * z, z, k1), q * d * d, s);
+    for (int e = 0; e < W; e += 2) {
+      // bounded as below; min and max drop a NaN, which is put back at the end
+      const float2 z = make_float2(fminf(fmaxf(pre[e], -16.0f), 16.0f), fminf(fmaxf(pre[e + 1], -16.0f), 16.0f));
+      float2 g;
+      const float2 s = normal_cdf_pair(z, g);
+      const float2 v = fma2(mul2(z, both(0.39894228040143268f)), g, s);
+      x[e] = pre[e] != pre[e] ? pre[e] : x[e] * v.x;
+      x[e + 1] = pre[e + 1] != pre[e + 1] ? pre[e + 1] : x[e + 1] * v.y;
     }
-    if (kAct == HC_ACT_GELU) {
-      float g;
-      const float s = normal_cdf<kFast>(z, g);
-      x[e] *= fmaf(z * 0.39894228040143268f, g, s);
+  } else {
+    constexpr float kBound = kAct == HC_ACT_SILU ? 80.0f : 16.0f;
+    constexpr float k1 = kAct == HC_ACT_SILU ? 1.0f : kTanh1, k3 = kAct == HC_ACT_SILU ? 0.0f : kTanh3;
+#pragma unroll
+    for (int e = 0; e < W; e++) {
+      if (kAct == HC_ACT_RELU) x[e] = pre[e] <= 0.0f ? 0.0f : x[e];
+      const float z = pre[e] != pre[e] ? pre[e] : fminf(fmaxf(pre[e], -kBound), kBound);
+      if (kAct == HC_ACT_SILU || kAct == HC_ACT_GELU_TANH) {
+        const float q = exp_f<kFast>(-1.0f, fabsf(z) * fmaf(k3 * z, z, k1));   // in (0, 1]: both sigmas from it
+        const float d = recip_f<kFast>(1.0f + q);
+        const float s = z < 0.0f ? q * d : d;
+        x[e] *= fmaf(z * fmaf(3.0f * k3 * z, z, k1), q * d * d, s);
+      }
+      if (kAct == HC_ACT_GELU) {
+        float g;
+        const float s = normal_cdf<kFast>(z, g);
+        x[e] *= fmaf(z * 0.39894228040143268f, g, s);
+      }
     }
   }
 }

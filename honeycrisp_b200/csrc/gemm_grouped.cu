@@ -6,7 +6,7 @@
 //
 // The offsets stay on the device: group_setup_kernel turns them into a table of tiles, which the persistent CTAs of
 // the product walk, so the host neither waits for the router nor launches once a group, and a captured graph
-// follows new offsets.  Offsets that leave [0, total_rows] or run backwards are clamped there, so that no table can
+// follows new offsets.  Groups of few rows take CUDA-core forms where those read or write less (gemm_skinny.cu).  Offsets that leave [0, total_rows] or run backwards are clamped there, so that no table can
 // send a copy out of range.
 #include "tc_kernel.cuh"
 
@@ -205,6 +205,31 @@ cudaError_t launch_grouped(const GroupedProblem& p, cudaStream_t stream, unsigne
   const int eb = f32 ? 4 : 2, BK = 128 / eb;
   *rec = LaunchRecord();
   rec->kernel = HC_KERNEL_TENSOR;
+  auto setup = [&](int* start, int tile_rows, int tiles_n, int64_t per_group) {
+    const int64_t* offsets = p.offsets;
+    int groups = (int)p.groups, per = (int)per_group;
+    int64_t total = p.total_rows;
+    int *end = start + groups, *first_tile = end + groups;
+    void* args[] = {(void*)&offsets, (void*)&groups, (void*)&total, (void*)&tile_rows, (void*)&tiles_n, (void*)&per, (void*)&start, (void*)&end, (void*)&first_tile};
+    rec->launches++;
+    return launch_behind((const void*)group_setup_kernel, args, dim3(1), dim3(1024), 0, stream);
+  };
+  if (few_preferred(p)) {
+    const size_t need = round256((size_t)(3 * p.groups + 1) * sizeof(int));
+    *scratch_needed = need;
+    if (!scratch || scratch_bytes < need) return cudaErrorInvalidValue;
+    const int strips = few_strips(p);
+    const int64_t tiles = (p.total_rows / 8 + p.groups) * strips;   // forward: at most
+    if (tiles >= (1ll << 31) || p.total_rows >= (1ll << 31) - 256) return cudaErrorNotSupported;
+    int* start = (int*)scratch;
+    cudaError_t e = setup(start, 8, strips, wg ? 1 : 0);
+    if (e != cudaSuccess) return e;
+    const GroupTiles t = {start, start + p.groups, start + 2 * p.groups, (int)p.groups};
+    rec->kernel = HC_KERNEL_SIMT;
+    rec->tile_m = 8; rec->tiles = tiles; rec->scratch_bytes = need;
+    rec->launches++;
+    return launch_few(p, t, tiles, stream);
+  }
   // Result rows and columns of a group, and the contracted length: the group's rows for the weight gradient.
   const int64_t m = wg ? p.rows : p.total_rows, n = p.cols;
   const int64_t mean_rows = (p.total_rows + p.groups - 1) / p.groups;
@@ -246,15 +271,8 @@ cudaError_t launch_grouped(const GroupedProblem& p, cudaStream_t stream, unsigne
 
   cudaError_t e = empty ? cudaSuccess : launch_operands(a, b, eb, stream, rec);
   if (e != cudaSuccess) return e;
-  {
-    const int64_t* offsets = p.offsets;
-    int groups = (int)p.groups, rows = tp.tile_rows, tn = tp.tiles_n, per = (int)per_group;
-    int64_t total = p.total_rows;
-    void* args[] = {(void*)&offsets, (void*)&groups, (void*)&total, (void*)&rows, (void*)&tn, (void*)&per, (void*)&start, (void*)&end, (void*)&first_tile};
-    e = launch_behind((const void*)group_setup_kernel, args, dim3(1), dim3(1024), 0, stream);
-    if (e != cudaSuccess) return e;
-    rec->launches++;
-  }
+  e = setup(start, tp.tile_rows, tp.tiles_n, per_group);
+  if (e != cudaSuccess) return e;
   if (empty) {
     void* out = p.out;
     int64_t cols = p.cols;

@@ -5,7 +5,7 @@
 // matrices that the kernel behind sums in ascending order, with the epilogue.
 // Where it is taken (skinny_preferred), measured at 4096 x 16384 weights: float32, which the tensor cores take as two halves
 // written by a pass of their own (4 rows: 57 us here, 200 there); weights that TMA cannot address, which would be copied whole
-// first (4 rows of 4095 x 16383 float16: 48 us, 271); one row of float16 (25.7 us whatever the activation, 26 to 28 there;
+// first (4 rows of 4095 x 16383 float16: 67 us, 101); one row of float16 (25.7 us whatever the activation, 26 to 28 there;
 // the floor is 20.5).  Two to eight rows of float16 are the tensor cores' (4 rows: 48 us here, 26 there).
 // It also takes the small products of few rows that one 128 x 128 CUDA-core tile would walk alone (1024 x 1024, one row:
 // 12 us for 305).
@@ -24,44 +24,38 @@ struct SkinnyJob {
   int chunk;            // contracted indices a part
 };
 
-template <typename T, int kM>
-__device__ __forceinline__ void stage_x(const SkinnyJob& j, float* xs, int64_t k0, int n, bool k_inner) {
-  // xs[k][m] for the column-wise kernel, xs[m][k] for the row-wise one
+// Rows of x, widened, in shared memory: xs[k][m] for the column-wise form, xs[m][k] (pitch kMaxChunk) for the row-wise one.
+template <typename T, int kM, bool kRowWise>
+__device__ __forceinline__ void stage_x(float* xs, const T* x, int64_t ldx, int rows, int n) {
   for (int i = threadIdx.x; i < kM * n; i += 256) {
     const int m = i / n, k = i - m * n;
-    xs[k_inner ? m * kMaxChunk + k : k * kM + m] = widen_f<T>(((const T*)j.x)[m * j.ldx + k0 + k]);
+    xs[kRowWise ? m * kMaxChunk + k : k * kM + m] = m < rows ? widen_f<T>(x[m * ldx + k]) : 0.0f;
+  }
+}
+template <int kM>
+__device__ __forceinline__ void read_x(const float* xs, int k, float (&x)[kM]) {
+  if constexpr (kM % 4 == 0) {
+#pragma unroll
+    for (int q = 0; q < kM / 4; q++) {
+      const float4 v = *(const float4*)(xs + k * kM + q * 4);
+      x[q * 4] = v.x; x[q * 4 + 1] = v.y; x[q * 4 + 2] = v.z; x[q * 4 + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int m = 0; m < kM; m++) x[m] = xs[k * kM + m];
   }
 }
 
-// w stored [K][N]: a thread owns eight columns (adjacent where 16-byte loads allow it, else 64 apart, so that a warp's loads
-// are adjacent), four groups of 64 threads take every fourth row of the part.
+// w stored [K][N], from the CTA's first row and column on: a thread owns eight columns (adjacent where 16-byte loads allow it,
+// else 64 apart, so that a warp's loads are adjacent), four groups of 64 threads take every fourth of the `n` rows.
 template <typename T, int kM, bool kVec>
-__global__ void __launch_bounds__(256) skinny_columns_kernel(const SkinnyJob j) {
-  extern __shared__ __align__(16) float smem[];
-  pdl_wait();
-  pdl_release();
+__device__ __forceinline__ void walk_columns(const T* w, int64_t ldw, int64_t cols, const float* xs, int n, float (&acc)[kM][8]) {
   const int tx = threadIdx.x % 64, ky = threadIdx.x / 64;
-  const int64_t k0 = (int64_t)blockIdx.y * j.chunk;
-  const int n = (int)min((int64_t)j.chunk, j.K - k0);
-  const int64_t col0 = (int64_t)blockIdx.x * 512;
-  stage_x<T, kM>(j, smem, k0, n, false);
-  __syncthreads();
-  float acc[kM][8];
-#pragma unroll
-  for (int m = 0; m < kM; m++)
-#pragma unroll
-    for (int e = 0; e < 8; e++) acc[m][e] = 0.0f;
-  const T* w = (const T*)j.w + k0 * j.ldw + col0 + (kVec ? tx * 8 : tx);
-  bool in[kVec ? 1 : 8];
-  if (kVec) in[0] = col0 + tx * 8 < j.N;
-  else
-#pragma unroll
-    for (int e = 0; e < 8; e++) in[e % (kVec ? 1 : 8)] = col0 + tx + 64 * e < j.N;
+  w += kVec ? tx * 8 : tx;
   constexpr int kAhead = kVec ? (sizeof(T) == 2 ? 8 : 4) : 2;   // rows whose loads are under way together
   auto row = [&](int k, const float (&v)[8]) {
     float x[kM];
-#pragma unroll
-    for (int m = 0; m < kM; m++) x[m] = smem[k * kM + m];
+    read_x<kM>(xs, k, x);
 #pragma unroll
     for (int m = 0; m < kM; m++)
 #pragma unroll
@@ -70,12 +64,13 @@ __global__ void __launch_bounds__(256) skinny_columns_kernel(const SkinnyJob j) 
   for (int kb = ky; kb < n; kb += 4 * kAhead) {
     if constexpr (kVec) {
       constexpr int kPieces = sizeof(T) == 2 ? 1 : 2;
+      const bool in = tx * 8 < cols;
       uint4 u[kAhead][kPieces];
 #pragma unroll
       for (int i = 0; i < kAhead; i++)
 #pragma unroll
         for (int q = 0; q < kPieces; q++)
-          u[i][q] = kb + 4 * i < n && in[0] ? __ldcs((const uint4*)(w + (int64_t)(kb + 4 * i) * j.ldw) + q) : make_uint4(0, 0, 0, 0);
+          u[i][q] = kb + 4 * i < n && in ? __ldcs((const uint4*)(w + (int64_t)(kb + 4 * i) * ldw) + q) : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < kAhead; i++) {
         if (kb + 4 * i >= n) break;
@@ -96,7 +91,7 @@ __global__ void __launch_bounds__(256) skinny_columns_kernel(const SkinnyJob j) 
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           T t = (T)0.0f;
-          if (kb + 4 * i < n && in[e]) t = w[(int64_t)(kb + 4 * i) * j.ldw + 64 * e];
+          if (kb + 4 * i < n && tx + 64 * e < cols) t = w[(int64_t)(kb + 4 * i) * ldw + 64 * e];
           u[i][e] = t;
         }
 #pragma unroll
@@ -109,106 +104,144 @@ __global__ void __launch_bounds__(256) skinny_columns_kernel(const SkinnyJob j) 
       }
     }
   }
-  // the four groups' sums, over the rows in shared memory
+}
+// The four groups' sums through shared memory (over the staged rows); `out(m, column of the strip, sum)` for the first group's.
+template <int kM, bool kVec, typename F>
+__device__ __forceinline__ void join_columns(float* red, const float (&acc)[kM][8], F&& out) {
+  const int tx = threadIdx.x % 64, ky = threadIdx.x / 64;
   __syncthreads();
-  float* red = smem;   // [3][kM][512]
   if (ky > 0)
 #pragma unroll
     for (int m = 0; m < kM; m++)
 #pragma unroll
-      for (int e = 0; e < 8; e++) red[((ky - 1) * kM + m) * 512 + (kVec ? e * 64 + tx : tx + 64 * e)] = acc[m][e];
+      for (int e = 0; e < 8; e++) red[((ky - 1) * kM + m) * 512 + e * 64 + tx] = acc[m][e];
   __syncthreads();
-  if (ky > 0) return;
+  if (ky == 0)
 #pragma unroll
-  for (int m = 0; m < kM; m++)
+    for (int m = 0; m < kM; m++)
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      float s = acc[m][e];
+      for (int e = 0; e < 8; e++) {
+        float s = acc[m][e];
 #pragma unroll
-      for (int g = 0; g < 3; g++) s += red[(g * kM + m) * 512 + e * 64 + tx];
-      const int64_t col = col0 + (kVec ? tx * 8 + e : tx + 64 * e);
-      if (col < j.N) j.ws[((int64_t)blockIdx.y * kM + m) * j.ws_ld + col] = s;
-    }
+        for (int g = 0; g < 3; g++) s += red[(g * kM + m) * 512 + e * 64 + tx];
+        out(m, kVec ? tx * 8 + e : tx + 64 * e, s);
+      }
 }
 
-// w stored [N][K]: a warp takes four columns at a time along the part, a lane eight adjacent contracted indices (or eight 32 apart).
+// w stored [N][K], from a warp's first of four columns on: a lane takes eight adjacent contracted indices (or eight 32 apart).
+constexpr int kCols = 4;
+template <typename T, int kM, bool kVec>
+__device__ __forceinline__ void walk_rows(const T* w0, int64_t ldw, int64_t cols, const float* xs0, int n, float (&acc)[kCols][kM]) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll 2
+  for (int kb = 0; kb < n; kb += 256) {
+    float v[kCols][8];
+    const T* w = w0 + kb;
+    if constexpr (kVec) {
+      constexpr int kPieces = sizeof(T) == 2 ? 1 : 2, E = 8 / kPieces;
+      uint4 u[kCols][kPieces];
+#pragma unroll
+      for (int c = 0; c < kCols; c++)
+#pragma unroll
+        for (int q = 0; q < kPieces; q++)
+          u[c][q] = c < cols && kb + lane * 8 < n ? __ldcs((const uint4*)(w + c * ldw + lane * 8) + q) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < kCols; c++)
+#pragma unroll
+        for (int q = 0; q < kPieces; q++) {
+          float part[E];
+          Pack16<T>::widen(u[c][q], part);
+#pragma unroll
+          for (int e = 0; e < E; e++) v[c][q * E + e] = part[e];
+        }
+    } else {
+      T u[kCols][8];
+#pragma unroll
+      for (int c = 0; c < kCols; c++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          T t = (T)0.0f;
+          if (c < cols && kb + lane + 32 * e < n) t = w[c * ldw + lane + 32 * e];
+          u[c][e] = t;
+        }
+#pragma unroll
+      for (int c = 0; c < kCols; c++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[c][e] = widen_f<T>(u[c][e]);
+    }
+#pragma unroll
+    for (int m = 0; m < kM; m++) {
+      float x[8];
+      const float* xs = xs0 + m * kMaxChunk + kb;
+      if (kVec && kb + lane * 8 < n) {   // n is a multiple of eight here
+        const float4 a = *(const float4*)(xs + lane * 8), b = *(const float4*)(xs + lane * 8 + 4);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = !kVec && kb + lane + 32 * e < n ? xs[lane + 32 * e] : 0.0f;   // beyond, the buffer holds nothing
+      }
+#pragma unroll
+      for (int c = 0; c < kCols; c++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc[c][m] = fmaf(x[e], v[c][e], acc[c][m]);
+    }
+  }
+}
+template <int kM, typename F>
+__device__ __forceinline__ void join_rows(float (&acc)[kCols][kM], F&& out) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int c = 0; c < kCols; c++)
+#pragma unroll
+    for (int m = 0; m < kM; m++) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) acc[c][m] += __shfl_xor_sync(0xffffffffu, acc[c][m], o);
+      if (lane == c * kM + m) out(m, c, acc[c][m]);
+    }
+}
+template <int kA, int kB>
+__device__ __forceinline__ void clear(float (&acc)[kA][kB]) {
+#pragma unroll
+  for (int a = 0; a < kA; a++)
+#pragma unroll
+    for (int b = 0; b < kB; b++) acc[a][b] = 0.0f;
+}
+
+template <typename T, int kM, bool kVec>
+__global__ void __launch_bounds__(256) skinny_columns_kernel(const SkinnyJob j) {
+  extern __shared__ __align__(16) float smem[];
+  pdl_wait();
+  pdl_release();
+  const int64_t k0 = (int64_t)blockIdx.y * j.chunk, col0 = (int64_t)blockIdx.x * 512;
+  const int n = (int)min((int64_t)j.chunk, j.K - k0);
+  stage_x<T, kM, false>(smem, (const T*)j.x + k0, j.ldx, kM, n);
+  __syncthreads();
+  float acc[kM][8];
+  clear(acc);
+  walk_columns<T, kM, kVec>((const T*)j.w + k0 * j.ldw + col0, j.ldw, j.N - col0, smem, n, acc);
+  join_columns<kM, kVec>(smem, acc, [&](int m, int c, float s) {
+    if (col0 + c < j.N) j.ws[((int64_t)blockIdx.y * kM + m) * j.ws_ld + col0 + c] = s;
+  });
+}
+
 template <typename T, int kM, bool kVec>
 __global__ void __launch_bounds__(256) skinny_rows_kernel(const SkinnyJob j, int columns_per_warp) {
   extern __shared__ __align__(16) float smem[];
   pdl_wait();
   pdl_release();
-  constexpr int kCols = 4;
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int warp = threadIdx.x / 32;
   const int64_t k0 = (int64_t)blockIdx.y * j.chunk;
   const int n = (int)min((int64_t)j.chunk, j.K - k0);
-  stage_x<T, kM>(j, smem, k0, n, true);
+  stage_x<T, kM, true>(smem, (const T*)j.x + k0, j.ldx, kM, n);
   __syncthreads();
   const int64_t first = ((int64_t)blockIdx.x * 8 + warp) * columns_per_warp;
   for (int64_t c0 = first; c0 < min(first + columns_per_warp, j.N); c0 += kCols) {
     float acc[kCols][kM];
-#pragma unroll
-    for (int c = 0; c < kCols; c++)
-#pragma unroll
-      for (int m = 0; m < kM; m++) acc[c][m] = 0.0f;
-#pragma unroll 2
-    for (int kb = 0; kb < n; kb += 256) {
-      float v[kCols][8];
-      const T* w = (const T*)j.w + c0 * j.ldw + k0 + kb;
-      if constexpr (kVec) {
-        constexpr int kPieces = sizeof(T) == 2 ? 1 : 2, E = 8 / kPieces;
-        uint4 u[kCols][kPieces];
-#pragma unroll
-        for (int c = 0; c < kCols; c++)
-#pragma unroll
-          for (int q = 0; q < kPieces; q++)
-            u[c][q] = c0 + c < j.N && kb + lane * 8 < n ? __ldcs((const uint4*)(w + c * j.ldw + lane * 8) + q) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int c = 0; c < kCols; c++)
-#pragma unroll
-          for (int q = 0; q < kPieces; q++) {
-            float part[E];
-            Pack16<T>::widen(u[c][q], part);
-#pragma unroll
-            for (int e = 0; e < E; e++) v[c][q * E + e] = part[e];
-          }
-      } else {
-        T u[kCols][8];
-#pragma unroll
-        for (int c = 0; c < kCols; c++)
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            T t = (T)0.0f;
-            if (c0 + c < j.N && kb + lane + 32 * e < n) t = w[c * j.ldw + lane + 32 * e];
-            u[c][e] = t;
-          }
-#pragma unroll
-        for (int c = 0; c < kCols; c++)
-#pragma unroll
-          for (int e = 0; e < 8; e++) v[c][e] = widen_f<T>(u[c][e]);
-      }
-#pragma unroll
-      for (int m = 0; m < kM; m++) {
-        float x[8];
-        const float* xs = smem + m * kMaxChunk + kb;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const int at = kVec ? lane * 8 + e : lane + 32 * e;
-          x[e] = kb + at < n ? xs[at] : 0.0f;   // beyond the part the buffer holds nothing
-        }
-#pragma unroll
-        for (int c = 0; c < kCols; c++)
-#pragma unroll
-          for (int e = 0; e < 8; e++) acc[c][m] = fmaf(x[e], v[c][e], acc[c][m]);
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < kCols; c++)
-#pragma unroll
-      for (int m = 0; m < kM; m++) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) acc[c][m] += __shfl_xor_sync(0xffffffffu, acc[c][m], o);
-        if (lane == c * kM + m && c0 + c < j.N) j.ws[((int64_t)blockIdx.y * kM + m) * j.ws_ld + c0 + c] = acc[c][m];
-      }
+    clear(acc);
+    walk_rows<T, kM, kVec>((const T*)j.w + c0 * j.ldw + k0, j.ldw, j.N - c0, smem, n, acc);
+    join_rows<kM>(acc, [&](int m, int c, float s) {
+      if (c0 + c < j.N) j.ws[((int64_t)blockIdx.y * kM + m) * j.ws_ld + c0 + c] = s;
+    });
   }
 }
 
@@ -269,6 +302,180 @@ bool skinny_fits(const GemmProblem& p) {
 bool skinny_preferred(const GemmProblem& p) {
   const bool addressable = ((uintptr_t)p.B & 15) == 0 && (p.ldb * 2) % 16 == 0;
   return p.dtype == HC_F32 || !addressable || p.M == 1;
+}
+
+// ---- the same for groups of rows -------------------------------------------------------------------------------------------
+namespace {
+
+// A tile is eight rows of a group by a strip of its matrix (512 columns, or 64 of the row-wise form); the table is
+// group_setup_kernel's.  The whole contraction is walked, in chunks of the staged rows.
+struct FewJob {
+  const void *a, *b;
+  void* out;
+  int64_t inner, cols;
+  GroupTiles t;
+  int strips;
+};
+template <typename T, bool kVec, bool kRowWise, int kM>
+__device__ __forceinline__ void few_tile(const FewJob& j, float* smem, int g, int64_t row0, int rows, int strip) {
+  const T* x = (const T*)j.a + row0 * j.inner;
+  const T* w = (const T*)j.b + (int64_t)g * j.inner * j.cols;
+  T* out = (T*)j.out + row0 * j.cols;
+  if constexpr (!kRowWise) {
+    const int64_t col0 = (int64_t)strip * 512;
+    float acc[kM][8];
+    clear(acc);
+    for (int64_t k0 = 0; k0 < j.inner; k0 += kMaxChunk) {
+      const int n = (int)min((int64_t)kMaxChunk, j.inner - k0);
+      __syncthreads();
+      stage_x<T, kM, false>(smem, x + k0, j.inner, rows, n);
+      __syncthreads();
+      walk_columns<T, kM, kVec>(w + k0 * j.cols + col0, j.cols, j.cols - col0, smem, n, acc);
+    }
+    join_columns<kM, kVec>(smem, acc, [&](int m, int c, float s) {
+      if (m < rows && col0 + c < j.cols) out[m * j.cols + col0 + c] = narrow_f<T>(s);
+    });
+  } else {
+    const int64_t first = (int64_t)strip * 64 + threadIdx.x / 32 * 8;
+    float acc[2][kCols][kM];
+#pragma unroll
+    for (int q = 0; q < 2; q++) clear(acc[q]);
+    for (int64_t k0 = 0; k0 < j.inner; k0 += kMaxChunk) {
+      const int n = (int)min((int64_t)kMaxChunk, j.inner - k0);
+      __syncthreads();
+      stage_x<T, kM, true>(smem, x + k0, j.inner, rows, n);
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < 2; q++)
+        if (first + 4 * q < j.cols) walk_rows<T, kM, kVec>(w + (first + 4 * q) * j.inner + k0, j.inner, j.cols - first - 4 * q, smem, n, acc[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < 2; q++)
+      join_rows<kM>(acc[q], [&](int m, int c, float s) {
+        if (m < rows && first + 4 * q + c < j.cols) out[m * j.cols + first + 4 * q + c] = narrow_f<T>(s);
+      });
+  }
+}
+template <typename T, bool kVec, bool kRowWise>
+__global__ void __launch_bounds__(256) few_rows_kernel(const FewJob j) {
+  extern __shared__ __align__(16) float smem[];
+  pdl_wait();
+  int lo = 0, hi = j.t.groups - 1;
+  if ((int)blockIdx.x >= j.t.first_tile[j.t.groups]) return;   // the grid is for the most tiles there could be
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (j.t.first_tile[mid] <= (int)blockIdx.x) lo = mid;
+    else hi = mid - 1;
+  }
+  const int r = (int)blockIdx.x - j.t.first_tile[lo], chunk = r / j.strips, strip = r - chunk * j.strips;
+  const int64_t row0 = j.t.start[lo] + 8 * chunk;
+  const int rows = min(8, (int)(j.t.end[lo] - row0));
+  if (rows <= 2) few_tile<T, kVec, kRowWise, 2>(j, smem, lo, row0, rows, strip);
+  else if (rows <= 4) few_tile<T, kVec, kRowWise, 4>(j, smem, lo, row0, rows, strip);
+  else few_tile<T, kVec, kRowWise, 8>(j, smem, lo, row0, rows, strip);
+}
+
+// Weight gradient: a CTA's 32 x 512 outputs, eight by eight a thread, summed over the group's rows 16 at a time from shared
+// memory.  Bound by writing the result, as long as the rows are few.
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(256) few_weight_grad_kernel(const void* a, const void* b, void* out, int64_t rows, int64_t cols, GroupTiles t) {
+  __shared__ __align__(16) float as[16][32], bs[16][512];
+  pdl_wait();
+  const int g = blockIdx.z, tx = threadIdx.x % 64, ty = threadIdx.x / 64;
+  const int64_t i0 = (int64_t)blockIdx.y * 32, j0 = (int64_t)blockIdx.x * 512;
+  const int start = t.start[g], n = t.end[g] - start;
+  float acc[8][8];
+  clear(acc);
+  for (int r0 = 0; r0 < n; r0 += 16) {
+    const int nr = min(16, n - r0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < nr * 32; i += 256) {
+      const int r = i / 32, c = i % 32;
+      as[r][c] = i0 + c < rows ? widen_f<T>(((const T*)a)[(start + r0 + r) * rows + i0 + c]) : 0.0f;
+    }
+    for (int i = threadIdx.x; i < nr * 512; i += 256) {
+      const int r = i / 512, c = i % 512;
+      bs[r][c] = j0 + c < cols ? widen_f<T>(((const T*)b)[(start + r0 + r) * cols + j0 + c]) : 0.0f;
+    }
+    __syncthreads();
+    for (int r = 0; r < nr; r++) {
+      float x[8], v[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        x[e] = as[r][ty * 8 + e];
+        v[e] = bs[r][kVec ? tx * 8 + e : tx + 64 * e];
+      }
+#pragma unroll
+      for (int p = 0; p < 8; p++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc[p][e] = fmaf(x[p], v[e], acc[p][e]);
+    }
+  }
+  T* dst = (T*)out + (int64_t)g * rows * cols;
+#pragma unroll
+  for (int p = 0; p < 8; p++) {
+    const int64_t i = i0 + ty * 8 + p;
+    if (i >= rows) break;
+    if constexpr (kVec) {
+      if (j0 + tx * 8 >= cols) continue;
+      constexpr int W = Pack16<T>::W;
+#pragma unroll
+      for (int q = 0; q < 8 / W; q++) {
+        float v[W];
+#pragma unroll
+        for (int e = 0; e < W; e++) v[e] = acc[p][q * W + e];
+        *(uint4*)(dst + i * cols + j0 + tx * 8 + q * W) = Pack16<T>::narrow(v);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (j0 + tx + 64 * e < cols) dst[i * cols + j0 + tx + 64 * e] = narrow_f<T>(acc[p][e]);
+    }
+  }
+}
+
+template <typename T>
+cudaError_t launch_few_typed(const GroupedProblem& p, const GroupTiles& t, int64_t tiles, cudaStream_t stream) {
+  if (p.weight_grad) {
+    const bool vec = ((uintptr_t)p.out & 15) == 0 && p.cols % 8 == 0;
+    const void *a = p.a, *b = p.b;
+    void* out = p.out;
+    int64_t rows = p.rows, cols = p.cols;
+    void* args[] = {(void*)&a, (void*)&b, (void*)&out, (void*)&rows, (void*)&cols, (void*)&t};
+    return launch_behind(vec ? (const void*)few_weight_grad_kernel<T, true> : (const void*)few_weight_grad_kernel<T, false>, args,
+                         dim3((unsigned)((cols + 511) / 512), (unsigned)((rows + 31) / 32), (unsigned)p.groups), dim3(256), 0, stream);
+  }
+  const int64_t ld = p.trans_b ? p.inner : p.cols;
+  const bool vec = ((uintptr_t)p.b & 15) == 0 && ld % 8 == 0;
+  FewJob j = {p.a, p.b, p.out, p.inner, p.cols, t, few_strips(p)};
+  void* args[] = {(void*)&j};
+  const void* fn = p.trans_b ? (vec ? (const void*)few_rows_kernel<T, true, true> : (const void*)few_rows_kernel<T, false, true>)
+                             : (vec ? (const void*)few_rows_kernel<T, true, false> : (const void*)few_rows_kernel<T, false, false>);
+  return launch_behind(fn, args, dim3((unsigned)tiles), dim3(256), 49152, stream);   // eight staged rows; three groups' sums
+}
+
+}  // namespace
+
+int few_strips(const GroupedProblem& p) { return (int)((p.cols + (p.trans_b ? 63 : 511)) / (p.trans_b ? 64 : 512)); }
+
+// Groups of few rows, on the average (the offsets are not known to the host).  Forward: where the tensor cores would first have the
+// weights copied or split, which reads and writes them once more each (57 experts of 1049 x 2832 float32, two rows each:
+// 545 us there, 151 here); weight gradient: while a sum over the rows costs less than writing the result
+// (104 groups of 312 x 1251 float32 over nine rows in all: 331 us there, 34 here), but for float16 that TMA can address (64 groups of
+// 1024 x 4096 over two rows each: 128 us there, 150 here).
+bool few_preferred(const GroupedProblem& p) {
+  const int64_t eb = p.dtype == HC_F16 ? 2 : 4, mean = (p.total_rows + p.groups - 1) / p.groups;
+  if (p.weight_grad) {
+    const bool by_tma = p.rows % 8 == 0 && p.cols % 8 == 0 && (((uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.out) & 15) == 0;
+    return (p.rows + 31) / 32 <= 65535 && (p.dtype == HC_F32 ? mean <= 16 : mean <= 8 && !by_tma);
+  }
+  const int64_t ld = p.trans_b ? p.inner : p.cols;
+  const bool addressable = ((uintptr_t)p.b & 15) == 0 && (ld * eb) % 16 == 0;
+  return mean <= 8 && p.inner > 0 && (p.dtype == HC_F32 || !addressable);
+}
+
+cudaError_t launch_few(const GroupedProblem& p, const GroupTiles& t, int64_t tiles, cudaStream_t stream) {
+  return p.dtype == HC_F16 ? launch_few_typed<__half>(p, t, tiles, stream) : launch_few_typed<float>(p, t, tiles, stream);
 }
 
 cudaError_t launch_skinny(const GemmProblem& p, cudaStream_t stream, void* scratch, size_t scratch_bytes, int sm_count, LaunchRecord* rec,

@@ -282,7 +282,7 @@ hc_status run_problem(hc_ctx* ctx, hc_kernel kernel, const hc::GemmProblem& p, i
     // and add, k ascending: bit-identical to BackendCPU.swift:1290-1300 for every flag combination).
     // A fused product, which no other arithmetic has to match, leaves the CUDA cores wherever their walk along the contraction (about
     // a microsecond for every eight of it) is longer than a tensor-core launch.
-    const bool big = p.fused ? p.K >= 32 && (p.M * p.N * p.K >= kAutoTensorMinWork || p.K >= 128)
+    const bool big = p.fused ? p.M * p.N * p.K >= kAutoTensorMinWork || p.K >= 128
                              : (p.M * p.N >= 64 * 64) && (p.M * p.N * p.K >= kAutoTensorMinWork) && p.K >= 32;
     chosen = (big && hc::tc_supported(p)) ? HC_KERNEL_TENSOR : HC_KERNEL_SIMT_EXACT;
   }

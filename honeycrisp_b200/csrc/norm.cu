@@ -13,26 +13,6 @@
 namespace hc {
 namespace {
 
-// Two float32 operations in one instruction; each lane rounds as its scalar form does.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(*(unsigned long long*)&r)
-      : "l"(*(const unsigned long long*)&a), "l"(*(const unsigned long long*)&b), "l"(*(const unsigned long long*)&c));
-  return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(*(unsigned long long*)&r) : "l"(*(const unsigned long long*)&a), "l"(*(const unsigned long long*)&b));
-  return r;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(*(unsigned long long*)&r) : "l"(*(const unsigned long long*)&a), "l"(*(const unsigned long long*)&b));
-  return r;
-}
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
-
 struct NormJob {
   const void* x;
   const void* grad;     // backward
