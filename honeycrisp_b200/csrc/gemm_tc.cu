@@ -363,7 +363,7 @@ TcKey make_key(const GemmProblem& p, const void* scratch, const void* status, vo
   k.sA = p.strideA; k.sB = p.strideB; k.sC = p.strideC; k.plan_M = p.plan_M; k.plan_N = p.plan_N;
   k.A = p.A; k.B = p.B; k.C = p.C; k.bias = p.bias; k.scratch = scratch; k.status = status;
   if (p.fused) {
-    k.fused = 1; k.act = p.fe.act; k.grad = p.fe.grad; k.aux = p.fe.aux; k.pre = p.fe.pre;
+    k.fused = 1; k.bias = p.fe.bias; k.act = p.fe.act; k.grad = p.fe.grad; k.aux = p.fe.aux; k.pre = p.fe.pre;
   }
   for (int i = 0; i < n_extra && i < kMaxOut - 1; i++) k.extra[i] = extra_out[i];
   return k;

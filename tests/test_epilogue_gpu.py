@@ -100,6 +100,42 @@ def test_few_columns_and_long_contractions(be, dtype, tb):
         forward_case(be, rows, inner, cols, dtype, "silu", True, True, False, tb=tb)
 
 
+def test_same_buffers_with_other_extras(be):
+    """Repeats with the same operands and result but another bias, residual, kept tensor or activation: nothing of an earlier call stays."""
+    import torch
+    rng = np.random.default_rng(6)
+    rows, inner, cols = 256, 256, 512
+    a, b, _, _ = operands(rng, rows, inner, cols, np.float16)
+    ad, bd = torch.from_numpy(a).cuda(), torch.from_numpy(b).cuda()
+    extras = [torch.from_numpy(rng.standard_normal(cols).astype(np.float16)).cuda() for _ in range(2)]
+    wide = [torch.from_numpy(rng.standard_normal((rows, cols)).astype(np.float16)).cuda() for _ in range(2)]
+    kept = [torch.zeros(rows, cols, dtype=torch.float16, device="cuda") for _ in range(2)]
+    out = torch.empty(rows, cols, dtype=torch.float16, device="cuda")
+    z = a.astype(np.float64) @ b.astype(np.float64)
+    err = ref.product_error(a, b, np.float16) + 2.0 ** -20
+    torch.cuda.synchronize()
+    for act in ("none", "relu"):
+        for bias in (None, *extras):
+            for res in (None, *wide):
+                for pre in (None, *kept):
+                    if pre is not None:
+                        pre.zero_()
+                        torch.cuda.synchronize()
+                    be.matmulEpilogue(ad, False, bd, False, rows, inner, cols, np.float16, activation=act, bias=bias, residual=res, pre=pre, out=out)
+                    be.sync()
+                    want = z if bias is None else z + bias.cpu().numpy().astype(np.float64)
+                    if pre is not None:
+                        ref.within(pre.cpu().numpy(), want, err, np.float16)
+                    want = ref.activation(want, act) + (0 if res is None else res.cpu().numpy().astype(np.float64))
+                    ref.within(out.cpu().numpy(), want, err, np.float16)
+    for grad in wide:
+        for act in ("relu", "silu"):
+            be.matmulEpilogue(ad, False, bd, False, rows, inner, cols, np.float16, activation=act, gradPre=grad, out=out)
+            be.sync()
+            d = ref.slope(grad.cpu().numpy().astype(np.float64), act)
+            ref.within(out.cpu().numpy(), z * d, err * 1.2 + np.abs(z) * 4e-5, np.float16)
+
+
 def test_two_contexts_at_once(be):
     """Two contexts on two streams, the same inputs, calls enqueued in turn: each has its own work area."""
     import torch
