@@ -280,9 +280,9 @@ hc_status run_problem(hc_ctx* ctx, hc_kernel kernel, const hc::GemmProblem& p, i
   if (kernel == HC_KERNEL_AUTO) {
     // Tiny products stay on the CUDA cores, in the reference's own arithmetic (separate multiply
     // and add, k ascending: bit-identical to BackendCPU.swift:1290-1300 for every flag combination).
-    // A fused product, which no other arithmetic has to match, leaves the CUDA cores wherever their walk along the contraction (about
-    // a microsecond for every eight of it) is longer than a tensor-core launch.
-    const bool big = p.fused ? p.M * p.N * p.K >= kAutoTensorMinWork || p.K >= 128
+    // A fused product, which no other arithmetic has to match, leaves the CUDA cores wherever their walk along the contraction (some
+    // four microseconds for every eight of it) is longer than a tensor-core launch: 48 x 121 x 20 float16 66 us there, 10 here.
+    const bool big = p.fused ? p.K > 16 || p.M * p.N * p.K >= kAutoTensorMinWork
                              : (p.M * p.N >= 64 * 64) && (p.M * p.N * p.K >= kAutoTensorMinWork) && p.K >= 32;
     chosen = (big && hc::tc_supported(p)) ? HC_KERNEL_TENSOR : HC_KERNEL_SIMT_EXACT;
   }

@@ -96,7 +96,7 @@ def test_cut_contractions(diag, monkeypatch, dtype):
 @pytest.mark.parametrize("tb", [False, True])
 def test_few_columns_and_long_contractions(be, dtype, tb):
     """A result of one to three columns over a long contraction: one tile, cut into parts."""
-    for rows, inner, cols in [(9, 256, 1), (16, 300, 3), (40, 2048, 2), (8, 1500, 1), (1, 40000, 5), (7, 1030, 640)]:
+    for rows, inner, cols in [(9, 17, 1), (48, 121, 20), (20, 16, 7), (9, 256, 1), (16, 300, 3), (40, 2048, 2), (8, 1500, 1), (1, 40000, 5), (7, 1030, 640)]:
         forward_case(be, rows, inner, cols, dtype, "silu", True, True, False, tb=tb)
 
 
