@@ -579,7 +579,7 @@ cudaError_t prepare_tc(const GemmProblem& p, unsigned int* status_word, void* sc
   TcLaunchFn fn = nullptr;
   if (p.fused && !cut) {
     if (f32 && !windowed) return cudaErrorInvalidValue;   // the fused epilogue is not built for the no-window debug mode
-    fn = fused_kernel(f32, shape);
+    fn = fused_kernel(f32, shape, kslabs, p.fe);
     if (!fn) return cudaErrorInvalidValue;
   } else if (!f32 && cut) {
     if (shape == SHAPE_PAIR_128) fn = TcConfig<2, 128, 4, 4, false, 2, 1, 2, true>::launch;

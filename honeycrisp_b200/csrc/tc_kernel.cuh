@@ -128,7 +128,7 @@ typedef cudaError_t (*TcLaunchFn)(const CUtensorMap maps[4], const OutMaps& outs
 enum Shape { SHAPE_AUTO = 0, SHAPE_WIDE, SHAPE_PAIR, SHAPE_C1_256, SHAPE_C1_128, SHAPE_PAIR_128, SHAPE_PAIR_64,
              SHAPE_COUNT };
 // The kernel with the fused epilogue for a tile shape (csrc/gemm_fused.cu); null where it is not built.
-TcLaunchFn fused_kernel(bool f32, int shape);
+TcLaunchFn fused_kernel(bool f32, int shape, int kslabs, const FusedEpilogue& fe);
 
 namespace {
 

@@ -84,6 +84,22 @@ def test_every_tile_shape(diag, monkeypatch, shape, dtype):
         forward_case(diag, rows, inner, cols, dtype, "gelu_tanh", True, True, True)
 
 
+@pytest.mark.parametrize("inner", [2048, 4100])
+def test_long_contractions_on_the_widest_tile(diag, monkeypatch, inner):
+    """256x256 tiles whose pipeline and epilogue change with the contraction's length, several tiles a CTA pair."""
+    monkeypatch.setenv("HC_TC_SHAPE", "2")
+    monkeypatch.setenv("HC_TC_SPLITS", "1")
+    for extras in [(True, False, False), (True, True, False), (True, False, True), (True, True, True)]:
+        forward_case(diag, 300, inner, 600, np.float16, "gelu", *extras)
+    rng = np.random.default_rng(inner)
+    a, b, _, _ = operands(rng, 300, inner, 600, np.float16)
+    pre = rng.standard_normal((300, 600)).astype(np.float16)
+    out = diag.matmulEpilogue(a, False, b, False, 300, inner, 600, np.float16, activation="silu", gradPre=pre)
+    d = ref.slope(pre.astype(np.float64), "silu")
+    z = a.astype(np.float64) @ b.astype(np.float64)
+    ref.within(out.onCPU(np.float16)[: 300 * 600], z * d, ref.product_error(a, b, np.float16) * np.abs(d) + np.abs(z) * 4e-5, np.float16)
+
+
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
 def test_cut_contractions(diag, monkeypatch, dtype):
     for parts in (2, 5):
