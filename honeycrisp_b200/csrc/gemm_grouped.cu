@@ -19,6 +19,7 @@ __global__ void __launch_bounds__(1024) group_setup_kernel(const int64_t* offset
                                                            int tiles_n, int tiles_per_group, int* start, int* end, int* first_tile) {
   __shared__ int warp_max[32], warp_sum[32];
   pdl_wait();
+  pdl_release();   // the kernel behind sets itself up meanwhile, and waits for this one before it reads the table
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   int reached = 0, tiles = 0;   // over the groups of earlier rounds: largest end, number of tiles
   for (int g0 = 0; g0 < groups; g0 += 1024) {
@@ -73,6 +74,7 @@ struct TailJob {
 template <typename T, int kSlab>
 __global__ void __launch_bounds__(256) group_tail_kernel(const TailJob ja, const TailJob jb, const int* start, const int* end) {
   pdl_wait();
+  pdl_release();
   const TailJob& j = blockIdx.z == 0 ? ja : jb;
   const int g = blockIdx.x;
   const int s = start[g], n = end[g] - s, rem = n % kSlab;
