@@ -140,3 +140,67 @@ def test_experts_forward_and_backward(be, dtype):
     # parameter to its type.
     assert (np.abs(after[1] - w[1] * (1 - 1e-5)) <= np.abs(w[1]) * (2.0 ** -25 + 2.0 ** -24 + (2.0 ** -11 if dtype == np.float16 else 0))).all()
     assert (after[[0, 2, 3, 4]] != w[[0, 2, 3, 4]]).mean() > 0.9
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_captured_training_step(be, dtype):
+    """Every operator of a step in one graph on a fresh context (its work area grows during the capture), replayed on new inputs: the
+    bits of the same calls made one by one."""
+    import torch
+    from honeycrisp_b200 import CUDABackend
+    tt = {np.float16: torch.float16, np.float32: torch.float32}[dtype]
+    rows, width, hidden, groups = 200, 136, 264, 3
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    new = lambda *s, t=tt, scale=1.0: (torch.randn(*s, generator=gen, device="cuda") * scale).to(t)  # noqa: E731
+    buf = dict(x=new(rows, width), g=new(rows, width), nw=new(width, t=torch.float32), nb=new(width, t=torch.float32), uw=new(width, hidden, scale=0.1),
+               ub=new(hidden), dw=new(hidden, width, scale=0.1), db=new(width), ew=new(groups, width, width, scale=0.1))
+    buf["offsets"] = torch.tensor([0, 50, 51, 190], device="cuda")
+
+    def tensors():
+        z = lambda *s, t=tt: torch.zeros(*s, dtype=t, device="cuda")  # noqa: E731
+        f = torch.float32
+        return dict(n=z(rows, width), mean=z(rows, t=f), rstd=z(rows, t=f), h=z(rows, hidden), pre=z(rows, hidden), out=z(rows, width),
+                    dpre=z(rows, hidden), gpre=z(rows, hidden), ubg=z(hidden, t=f), uwg=z(width, hidden), dwg=z(hidden, width), dn=z(rows, width),
+                    dx=z(rows, width), nwg=z(width, t=f), nbg=z(width, t=f), eo=z(rows, width), ewg=z(groups, width, width),
+                    m=z(width, hidden, t=f), v=z(width, hidden, t=f))
+
+    def calls(b, r, plan):
+        dt, k = dtype, dict(mark=False)
+        wrap = lambda t: b.wrap(t.data_ptr(), t.numel() * t.element_size())  # noqa: E731
+        b.layerNorm(buf["x"], buf["nw"], buf["nb"], rows, width, dt, out=r["n"], mean=r["mean"], rstd=r["rstd"], **k)
+        b.matmulEpilogue(r["n"], False, buf["uw"], False, rows, width, hidden, dt, activation="gelu", bias=buf["ub"], pre=r["pre"], out=r["h"], **k)
+        b.matmulEpilogue(r["h"], False, buf["dw"], False, rows, hidden, width, dt, bias=buf["db"], residual=buf["x"], out=r["out"], **k)
+        b.matmulEpilogue(buf["g"], False, buf["dw"], True, rows, width, hidden, dt, activation="gelu", gradPre=r["pre"], out=r["dpre"], **k)
+        b.activationGrad(r["h"], r["pre"], rows, hidden, dt, "silu", out=r["gpre"], biasGrad=r["ubg"], **k)
+        b.matmul(r["n"], True, r["dpre"], False, False, width, rows, hidden, dt, out=wrap(r["uwg"]), **k)
+        b.matmul(r["h"], True, buf["g"], False, False, hidden, rows, width, dt, out=wrap(r["dwg"]), **k)
+        b.matmul(r["dpre"], False, buf["uw"], True, False, rows, hidden, width, dt, out=wrap(r["dn"]), **k)
+        b.layerNormGrad(r["dn"], buf["x"], buf["nw"], r["mean"], r["rstd"], rows, width, dt, out=r["dx"], weightGrad=r["nwg"], biasGrad=r["nbg"], **k)
+        b.groupedMatmul(groups, buf["offsets"], buf["x"], buf["ew"], False, rows, width, width, dt, out=r["eo"], **k)
+        b.groupedMatmulWeightGrad(groups, buf["offsets"], buf["x"], buf["g"], rows, width, width, dt, out=r["ewg"], **k)
+        b.adamW(plan, 3, mark=False)
+
+    one, other = tensors(), tensors()
+    weights = [buf["uw"].clone(), buf["uw"].clone()]
+    plans = [be.adamWPlan([dict(param=w, grad=r["uwg"], moment1=r["m"], moment2=r["v"])]) for w, r in zip(weights, (one, other))]
+    fresh = CUDABackend(0)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    fresh.useStream(s.cuda_stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        calls(fresh, one, plans[0])
+    for _ in range(3):
+        buf["x"].copy_(new(rows, width))
+        buf["g"].copy_(new(rows, width))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        calls(be, other, plans[1])
+        be.sync()
+        for name in one:
+            assert torch.equal(one[name], other[name]), name
+        assert torch.equal(*weights)
+    del graph
+    fresh.checkDeviceStatus()
+    fresh.close()

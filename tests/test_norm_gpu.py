@@ -184,3 +184,33 @@ def test_repeats_are_bitwise_equal(be):
     for _ in range(3):
         c = [t.onCPU() for t in be.layerNormGrad(g, x, w, m, r, rows, cols, np.float16)]
         assert all(np.array_equal(p, q) for p, q in zip(a, c))
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("rows,cols", [(3, 256), (400, 1024), (5, 4096), (330, 2048), (2, 8192)])
+def test_rows_off_16_byte_boundaries(be, rows, cols, dtype):
+    """The same rows one element further on: element accesses, the forward pass's sums in another order."""
+    import torch
+    x, w, b, g = data(rows, cols, dtype)
+    tt = {np.float16: torch.float16, np.float32: torch.float32}[dtype]
+
+    def off(v):
+        t = torch.zeros(v.size + 1, dtype=tt, device="cuda")
+        t[1:] = torch.from_numpy(v.reshape(-1)).cuda()
+        return t[1:]
+
+    xt, gt, out, dx = off(x), off(g), off(x), off(x)
+    y, m, r, h = forward64(x, w, b, 1e-5)
+    torch.cuda.synchronize()
+    be.layerNorm(xt, w, b, rows, cols, dtype, out=out)
+    _, dw, db = be.layerNormGrad(gt, xt, w, m.astype(np.float32), r.astype(np.float32), rows, cols, dtype, out=dx)
+    be.sync()
+    _, er, eh = forward_errors(x, h, r)
+    ref.within(out.cpu().numpy(), y, eh * np.abs(w) + (np.abs(h * w) + np.abs(y)) * 2.0 ** -23, dtype)
+    want = be.layerNormGrad(g, x, w, m.astype(np.float32), r.astype(np.float32), rows, cols, dtype)
+    # two orders of the same float32 sums
+    room = np.abs(g.astype(np.float64) * w).mean(1)[:, None] * (1 + np.abs(h)) * r[:, None] * 4 * sum_error(cols) + np.abs(g * w) * r[:, None] * 2.0 ** -21
+    ref.within(dx.cpu().numpy(), want[0].onCPU(dtype)[: rows * cols].astype(np.float64), room + 2 * ref.HALF_STEP[dtype] * np.abs(want[0].onCPU(dtype)[: rows * cols].reshape(rows, cols).astype(np.float64)), dtype)
+    sums = np.abs(g.astype(np.float64) * h).sum(0) * (rows * 2.0 ** -23 + 2.0 ** -21)
+    ref.within(dw.onCPU(np.float32)[:cols], want[1].onCPU(np.float32)[:cols].astype(np.float64), sums + np.abs(g).astype(np.float64).sum(0) * 2.0 ** -22, np.float32)
+    ref.within(db.onCPU(np.float32)[:cols], want[2].onCPU(np.float32)[:cols].astype(np.float64), np.abs(g).astype(np.float64).sum(0) * rows * 2.0 ** -23, np.float32)
