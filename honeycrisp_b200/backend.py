@@ -15,6 +15,7 @@ Everything is computed by the CUDA library; nothing here has a CPU path.
 """
 from __future__ import annotations
 
+import bisect
 import ctypes
 import enum
 from typing import Optional
@@ -306,6 +307,7 @@ class AdamWPlan:
                     raise ValueError(f"AdamWPlan: {name} overlaps {last[other]}")
             if end > reach[written]:
                 reach[written], last[written] = end, name
+        self._written = sorted((start, end, name) for start, end, written, name in spans if written)   # disjoint
 
     def setGrad(self, index: int, grad) -> None:
         """Tensor `index` takes its gradient from `grad` (of the same type and length) from now on."""
@@ -314,6 +316,10 @@ class AdamWPlan:
         ptr, keep = self._backend._input(grad, gd, row.count, "grad")
         if isinstance(grad, np.ndarray):
             raise TypeError("AdamWPlan: grad must lie on the device")
+        if ptr and row.count:
+            at = bisect.bisect_left(self._written, (ptr + row.count * gd.byteSize,))
+            if at and self._written[at - 1][1] > ptr:
+                raise ValueError(f"AdamWPlan: grad of tensor {index} overlaps {self._written[at - 1][2]}")
         row.grad = ptr or None
         self._grads[index] = keep
 
@@ -378,7 +384,8 @@ class CUDABackend:
         raise KernelFailed(msg)
 
     def useStream(self, cuda_stream_ptr: Optional[int]):
-        """Enqueue this backend's work on a stream owned by the caller (None: its own)."""
+        """Enqueue this backend's work on a stream owned by the caller (None or 0: its own).  torch's default stream is 1, the
+        legacy default stream, although torch gives its handle as 0; other torch streams go by their `cuda_stream`."""
         self._check(self._lib.hc_set_stream(self._ctx, cuda_stream_ptr or None))
 
     def enqueueWait(self, transfer: "ReadBack"):
@@ -606,7 +613,8 @@ class CUDABackend:
     # -- a feed-forward block ----------------------------------------------------------------
     # Tensors of these calls are device buffers (CUDAData), contiguous CUDA torch tensors, or, for inputs,
     # numpy arrays, which are staged.  Sizes are checked here; what the library refuses (overlaps, misaligned
-    # addresses, unknown activations, ranges of the scalars) raises ValueError.
+    # addresses, unknown activations, ranges of the scalars) raises ValueError.  Nothing here orders the backend's stream after
+    # torch's: run on torch's (useStream), or synchronise where tensors change hands and keep torch inputs alive until then.
 
     def _float_dtype(self, dtype, what: str):
         dt = _as_dtype(dtype)
@@ -622,6 +630,8 @@ class CUDABackend:
         if type(x) is CUDAData:
             if x.byteCount < count * dt.byteSize:
                 raise ValueError(f"{what} is smaller than its {count} elements")
+            if x.backend is not self and x.backend.device != self.device:
+                raise ValueError(f"{what} lies on device {x.backend.device}, the backend on device {self.device}")
             return x.ptr, x
         if hasattr(x, "element_size"):   # a torch tensor
             if _TORCH_DTYPE.get(x.dtype) is not dt and _torch_dtype(x.dtype) is not dt:
@@ -650,11 +660,15 @@ class CUDABackend:
         return ptr, x
 
     def _done(self, results, inputs, mark: bool):
+        """Keeps operands alive until the result is collected: those that belong to somebody else.  This backend's own buffers are
+        freed in the order of its stream and need no keeping, or a loop that feeds each result to the next call would keep
+        them all."""
         for r in results:
             if isinstance(r, CUDAData):
                 if mark:
                     r._mark()
-                r._inputs = inputs   # keep operands alive until the result is collected
+                r._inputs = tuple(k for k in inputs if k is not None and k is not r and
+                                  not (isinstance(k, CUDAData) and k._owns and k.backend is self))
 
     def _activation(self, name) -> int:
         try:

@@ -146,3 +146,47 @@ def test_adamw_plan_refuses_what_two_tensors_share(be):
         be.adamWPlan([row(param=B.CUDAData(be, 1 << 9, 32, owns=False)), row(moment1=B.CUDAData(be, (1 << 9) + 28, 32, owns=False))])
     be.adamWPlan([row(grad=grad), row(grad=grad)])       # a gradient is only read
     be.adamWPlan([row(param=B.CUDAData(be, 1 << 9, 32, owns=False)), row(param=B.CUDAData(be, (1 << 9) + 32, 32, owns=False))])
+
+
+def test_a_new_gradient_must_not_overlap_what_the_step_writes(be):
+    at = lambda p, n: B.CUDAData(be, p, n, owns=False)  # noqa: E731
+    row = lambda p: dict(param=at(p, 28), grad=at(p + 64, 28), moment1=at(p + 128, 28), moment2=at(p + 192, 28), dtype="float32", count=7)  # noqa: E731
+    plan = be.adamWPlan([row(4096), row(8192)])
+    for start in (4096, 4096 - 24, 4096 + 24, 8192 + 128, 8192 + 192 + 24):
+        with pytest.raises(ValueError, match="overlaps"):
+            plan.setGrad(0, at(start, 28))
+    assert plan._table[0].grad == 4096 + 64
+    for start in (4096 - 28, 4096 + 28, 8192 + 64, 1024, 1 << 20):
+        plan.setGrad(0, at(start, 28))
+        assert plan._table[0].grad == start
+
+
+def test_buffers_of_another_device_are_refused(be):
+    other = B.CUDABackend.__new__(B.CUDABackend)
+    other._lib, other._ctx, other.device = Recorder(), 1, 1
+    beside = B.CUDABackend.__new__(B.CUDABackend)
+    beside._lib, beside._ctx, beside.device = Recorder(), 1, 0
+    rest = (None, None, 2, 4, "float16")
+    with pytest.raises(ValueError, match="device 1"):
+        be.layerNorm(data(other, 8), *rest, out=data(be, 8), mark=False)
+    with pytest.raises(ValueError, match="device 1"):
+        be.layerNorm(data(be, 8), *rest, out=data(other, 8), mark=False)
+    be.layerNorm(data(beside, 8), *rest, out=data(be, 8), mark=False)
+    assert len(called(be, "hc_layer_norm")) == 1
+    other._ctx = beside._ctx = None
+
+
+def test_a_loop_keeps_no_earlier_results(be):
+    import weakref
+    owned = lambda n: B.CUDAData(be, 512, n * 2, owns=True)  # noqa: E731
+    borrowed, weight = data(be, 8), data(be, 16)
+    out = be.layerNorm(borrowed, None, None, 2, 4, "float16", out=owned(8), mark=False)
+    assert out._inputs == (borrowed,)
+    earlier = []
+    for _ in range(3):
+        earlier.append(weakref.ref(out))
+        out = be.matmulEpilogue(out, False, weight, False, 2, 4, 4, "float16", residual=out, out=owned(8), mark=False)
+        assert out._inputs == (weight,)
+    assert all(r() is None for r in earlier)
+    be.layerNorm(borrowed, None, None, 2, 4, "float16", out=borrowed, mark=False)   # in place: no cycle
+    assert borrowed._inputs == ()
