@@ -50,6 +50,8 @@ class DType(enum.Enum):
     float32 = "float32"
     int64 = "int64"  # legal in the reference's CPU backend; this backend throws notImplemented
 
+    __hash__ = object.__hash__   # members are singletons; Enum hashes their names, in Python
+
     @property
     def byteSize(self) -> int:
         return _BYTE_SIZE[self._value_]
@@ -91,6 +93,7 @@ def _torch_dtype(t) -> Optional[DType]:
 
 
 _HC_DTYPE = {DType.float16: L.HC_F16, DType.float32: L.HC_F32}
+_FLOAT = {}   # what callers name a float type by -> (DType, the library's number)
 
 
 class ReadBack:
@@ -617,10 +620,18 @@ class CUDABackend:
     # torch's: run on torch's (useStream), or synchronise where tensors change hands and keep torch inputs alive until then.
 
     def _float_dtype(self, dtype, what: str):
+        try:
+            return _FLOAT[dtype]
+        except (KeyError, TypeError):
+            pass
         dt = _as_dtype(dtype)
         hdt = _HC_DTYPE.get(dt)
         if hdt is None:
             raise NotImplementedByBackend(f"{what} for dtype {dt.value}")
+        try:
+            _FLOAT[dtype] = dt, hdt
+        except TypeError:
+            pass
         return dt, hdt
 
     def _input(self, x, dt: DType, count: int, what: str):
