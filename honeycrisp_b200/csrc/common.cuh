@@ -103,8 +103,6 @@ bool skinny_fits(const GemmProblem& p);
 bool skinny_preferred(const GemmProblem& p);   // to the tensor-core kernel
 cudaError_t launch_skinny(const GemmProblem& p, cudaStream_t stream, void* scratch, size_t scratch_bytes, int sm_count,
                           LaunchRecord* rec, size_t* scratch_needed);
-// result = epilogue(sum over parts of ws[part][M][ws_ld]), for a fused problem of one matrix.
-cudaError_t launch_sum_parts(const GemmProblem& p, const float* ws, int64_t ws_ld, int parts, cudaStream_t stream);
 // Another kernel has been launched on `stream`: the next product waits for it before it reads anything.
 void tc_forget_predecessor(cudaStream_t stream);
 // One-thread kernel whose bounded wait is made to expire after `limit_ns` (self-test).

@@ -5,8 +5,9 @@
 // matrices that the kernel behind sums in ascending order, with the epilogue.
 // Where it is taken (skinny_preferred), measured at 4096 x 16384 weights: float32, which the tensor cores take as two halves
 // written by a pass of their own (4 rows: 57 us here, 200 there); weights that TMA cannot address, which would be copied whole
-// first (4 rows of 4095 x 16383 float16: 67 us, 101); one row of float16 (25.7 us whatever the activation, 26 to 28 there;
-// the floor is 20.5).  Two to eight rows of float16 are the tensor cores' (4 rows: 48 us here, 26 there).
+// first (4 rows of 4095 x 16383 float16: 65 us, 101); one row of float16 (8192 x 8192 24.1 us here, 30.5 there; 4096 x 16384 23.5,
+// 26.7; 1000 x 50264 19.6, 25.0; 4096 x 1024 10.5, 10.0).  Two to eight rows of float16 are the tensor cores' (4 rows of the
+// 4096 x 16384: 48 us here, 26.7 there).
 // It also takes the small products of few rows that one 128 x 128 CUDA-core tile would walk alone (1024 x 1024, one row:
 // 12 us for 305).
 #include "epilogue.cuh"
@@ -245,6 +246,58 @@ __global__ void __launch_bounds__(256) skinny_rows_kernel(const SkinnyJob j, int
   }
 }
 
+// result = epilogue(sum over parts of ws[part][M][ws_ld]).  A lane takes four columns of a row; the CTA's warps (up to eight) take
+// every eighth part each, and their sums are added in order.  One thread walking all the parts, as where the tensor cores' few
+// parts are summed, would wait for them in turn (one row of 4096 x 1024 float32, 128 parts: 18.1 us for the product, 11.2 here).
+struct PartsJob {
+  const float* ws;
+  void* out;
+  int64_t M, N, ws_ld, ldc;
+  int parts, vec_ok;
+  FusedEpilogue fe;
+};
+constexpr int kPartWarps = 8;
+template <typename T>
+__global__ void __launch_bounds__(32 * kPartWarps) sum_parts_kernel(const PartsJob j) {
+  __shared__ float4 tile[kPartWarps][32];
+  pdl_release();
+  pdl_wait();
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+  const int64_t quads = j.ws_ld / 4, i = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t row = i / quads, n = (i - row * quads) * 4;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (row < j.M) {
+    const float* src = j.ws + row * j.ws_ld + n;
+    const int64_t pitch = j.M * j.ws_ld;
+#pragma unroll 4
+    for (int z = warp; z < j.parts; z += warps) {
+      const float4 v = __ldg((const float4*)(src + z * pitch));
+      acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+    }
+  }
+  if (warp > 0) tile[warp][lane] = acc;
+  __syncthreads();
+  if (warp > 0 || row >= j.M) return;
+  for (int w = 1; w < warps; w++) {
+    const float4 v = tile[w][lane];
+    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+  }
+  const int valid = (int)min((int64_t)4, j.N - n);
+  float x[4] = {acc.x, acc.y, acc.z, acc.w};
+  const int64_t off = row * j.ldc + n;
+  fused_direct<T, 4>(j.fe, off, n, valid, x);
+  T* dst = (T*)j.out + off;
+  T r[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) r[e] = narrow_f<T>(x[e]);
+  if (valid == 4 && j.vec_ok) {
+    if (sizeof(T) == 2) *(uint2*)dst = *(const uint2*)r;
+    else *(uint4*)dst = *(const uint4*)r;
+  } else {
+    for (int e = 0; e < valid; e++) dst[e] = r[e];
+  }
+}
+
 template <typename T, int kM>
 const void* pick(bool rows_form, bool vec) {
   if (rows_form) return vec ? (const void*)skinny_rows_kernel<T, kM, true> : (const void*)skinny_rows_kernel<T, kM, false>;
@@ -281,7 +334,10 @@ SkinnyPlan plan_skinny(const GemmProblem& p, int sm_count) {
   }
   int64_t parts = target / (s.strips > 0 ? s.strips : 1);
   if (parts > (p.K + least - 1) / least) parts = (p.K + least - 1) / least;
-  if (parts < (p.K + kMaxChunk - 1) / kMaxChunk) parts = (p.K + kMaxChunk - 1) / kMaxChunk;
+  const int64_t most = (p.K + kMaxChunk - 1) / kMaxChunk;   // parts that hold as much as a CTA can
+  // Where more CTAs are needed than run at once, the column-wise form takes whole rounds of them, just filled (8192 x 28672 float16,
+  // one row: 94 us with 448 CTAs, 72 with 840); the row-wise form, whose CTAs are shorter, loses by it (16384 x 4096 28.4, 32.5).
+  if (parts < most) parts = p.b_mn_major ? (most * s.strips + target - 1) / target * target / s.strips : most;
   if (parts < 1) parts = 1;
   int64_t chunk = (p.K + parts - 1) / parts;
   chunk = (chunk + 7) / 8 * 8;   // parts start where 16-byte loads of a row do
@@ -500,7 +556,12 @@ cudaError_t launch_skinny(const GemmProblem& p, cudaStream_t stream, void* scrat
   cudaError_t e = launch_behind(fn, args, dim3((unsigned)s.strips, (unsigned)s.parts), dim3(256), staged > sums ? staged : sums, stream);
   if (e != cudaSuccess) return e;
   rec->launches = 2;
-  return launch_sum_parts(p, (const float*)scratch, s.ws_ld, (int)s.parts, stream);
+  PartsJob sum = {(const float*)scratch, p.C, p.M, p.N, s.ws_ld, p.ldc, (int)s.parts, ((uintptr_t)p.C & (4 * eb - 1)) == 0 && p.ldc % 4 == 0, p.fe};
+  void* sum_args[] = {(void*)&sum};
+  const int warps = s.parts < kPartWarps ? (int)s.parts : kPartWarps;
+  const int64_t blocks = (p.M * (s.ws_ld / 4) + 31) / 32;
+  return launch_behind(p.dtype == HC_F16 ? (const void*)sum_parts_kernel<__half> : (const void*)sum_parts_kernel<float>, sum_args,
+                       dim3((unsigned)blocks), dim3(32 * warps), 0, stream);
 }
 
 }  // namespace hc

@@ -692,21 +692,6 @@ cudaError_t issue_tc(const TcPrepared& pp, int sm_count, cudaStream_t stream, La
 
 }  // namespace
 
-cudaError_t launch_sum_parts(const GemmProblem& p, const float* ws, int64_t ws_ld, int parts, cudaStream_t stream) {
-  ReduceJob job;
-  job.ws = ws; job.C = p.C; job.bias = nullptr;
-  job.M = p.M; job.N = p.N; job.ws_ld = ws_ld; job.batch = 1; job.parts = parts;
-  job.ldc = p.ldc; job.strideC = p.strideC;
-  job.fe = p.fe;
-  const bool f32 = p.dtype == HC_F32;
-  job.vec_ok = (((uintptr_t)p.C & (f32 ? 15 : 7)) == 0 && p.ldc % 4 == 0) ? 1 : 0;
-  int64_t blocks = (p.M * (ws_ld / 4) + 255) / 256;
-  if (blocks > 148 * 8) blocks = 148 * 8;
-  void* args[1] = {(void*)&job};
-  return launch_elementwise(f32 ? (const void*)splitk_reduce_kernel<false, true> : (const void*)splitk_reduce_kernel<true, true>, args,
-                            (int)blocks, stream);
-}
-
 void tc_forget_predecessor(cudaStream_t stream) {
   std::lock_guard<std::mutex> lock(g_track_mu);
   StreamTrack* t = track_entry(stream, false);

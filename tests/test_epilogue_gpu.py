@@ -359,3 +359,22 @@ def test_replayed_graph_and_growth_of_the_work_area(be):
     del g
     fresh.checkDeviceStatus()
     fresh.close()
+
+
+@pytest.mark.parametrize("shape", [0, 1, 2, 3, 4, 5, 6])
+@pytest.mark.parametrize("rows", [2, 3, 7, 8, 9, 15, 16, 17, 33, 131, 160 + 8, 256 + 12])
+def test_warps_with_few_rows(diag, monkeypatch, rows, shape):
+    """Tiles whose last 32 rows hold one to sixteen: their columns are shared among the lanes; with and without TMA, every extra, the gradient."""
+    if shape:
+        monkeypatch.setenv("HC_TC_SHAPE", str(shape))
+    monkeypatch.setenv("HC_TC_SPLITS", "1")
+    for cols in (72, 520, 517):
+        for act, extras in (("gelu", (True, False, False)), ("silu", (False, True, True)), ("none", (True, True, False)), ("relu", (False, False, True))):
+            forward_case(diag, rows, 136, cols, np.float16, act, *extras, tb=cols == 520)
+        rng = np.random.default_rng(rows + cols)
+        a, b, _, _ = operands(rng, rows, 136, cols, np.float16)
+        pre = rng.standard_normal((rows, cols)).astype(np.float16)
+        out = diag.matmulEpilogue(a, False, b, False, rows, 136, cols, np.float16, activation="gelu_tanh", gradPre=pre)
+        d = ref.slope(pre.astype(np.float64), "gelu_tanh")
+        z = a.astype(np.float64) @ b.astype(np.float64)
+        ref.within(out.onCPU(np.float16)[: rows * cols], z * d, ref.product_error(a, b, np.float16) * np.abs(d) + np.abs(z) * 4e-5, np.float16)
