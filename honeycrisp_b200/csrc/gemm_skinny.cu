@@ -53,14 +53,20 @@ template <typename T, int kM, bool kVec>
 __device__ __forceinline__ void walk_columns(const T* w, int64_t ldw, int64_t cols, const float* xs, int n, float (&acc)[kM][8]) {
   const int tx = threadIdx.x % 64, ky = threadIdx.x / 64;
   w += kVec ? tx * 8 : tx;
-  constexpr int kAhead = kVec ? (sizeof(T) == 2 ? 8 : 4) : 2;   // rows whose loads are under way together
+  // Rows whose loads are under way together; single elements of few rows want more of them (4095 x 16383 float16: one row 55.7 us with
+  // two, 38.5 with four; four rows 44.7, 55.9).
+  constexpr int kAhead = kVec ? (sizeof(T) == 2 ? 8 : 4) : kM <= 2 ? 4 : 2;
   auto row = [&](int k, const float (&v)[8]) {
     float x[kM];
     read_x<kM>(xs, k, x);
 #pragma unroll
     for (int m = 0; m < kM; m++)
 #pragma unroll
-      for (int e = 0; e < 8; e++) acc[m][e] = fmaf(x[m], v[e], acc[m][e]);
+      for (int e = 0; e < 8; e += 2) {
+        const float2 s = fma2(both(x[m]), make_float2(v[e], v[e + 1]), make_float2(acc[m][e], acc[m][e + 1]));
+        acc[m][e] = s.x;
+        acc[m][e + 1] = s.y;
+      }
   };
   for (int kb = ky; kb < n; kb += 4 * kAhead) {
     if constexpr (kVec) {
@@ -188,17 +194,30 @@ __device__ __forceinline__ void walk_rows(const T* w0, int64_t ldw, int64_t cols
     }
   }
 }
+// The lanes' sums: the butterfly halves the values while it halves the lanes, so that 32 of them take 31 shuffles, not 160.
 template <int kM, typename F>
 __device__ __forceinline__ void join_rows(float (&acc)[kCols][kM], F&& out) {
+  constexpr int kV = kCols * kM, kN = kV <= 4 ? 4 : kV <= 8 ? 8 : kV <= 16 ? 16 : 32, kShare = 32 / kN;   // lanes that end with the same sum
   const int lane = threadIdx.x % 32;
+  float v[kN];
 #pragma unroll
-  for (int c = 0; c < kCols; c++)
+  for (int i = 0; i < kN; i++) v[i] = i < kV ? acc[i < kV ? i / kM : 0][i % kM] : 0.0f;
+  int o = 16;
 #pragma unroll
-    for (int m = 0; m < kM; m++) {
+  for (int n = kN / 2; n >= 1; n >>= 1) {
+    const bool up = (lane & o) != 0;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) acc[c][m] += __shfl_xor_sync(0xffffffffu, acc[c][m], o);
-      if (lane == c * kM + m) out(m, c, acc[c][m]);
+    for (int i = 0; i < n; i++) {
+      const float send = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
     }
+    o >>= 1;
+  }
+  float x = v[0];
+#pragma unroll
+  for (int k = kShare / 2; k > 0; k >>= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
+  const int i = lane / kShare;
+  if (lane % kShare == 0 && i < kV) out(i % kM, i / kM, x);
 }
 template <int kA, int kB>
 __device__ __forceinline__ void clear(float (&acc)[kA][kB]) {
