@@ -4,8 +4,8 @@
 // cores; the contraction is cut so that about three CTAs an SM have 16-byte loads in flight, and the parts go to float32 partial
 // matrices that the kernel behind sums in ascending order, with the epilogue.
 // Where it is taken (skinny_preferred), measured at 4096 x 16384 weights: float32, which the tensor cores take as two halves
-// written by a pass of their own (4 rows: 57 us here, 200 there); weights that TMA cannot address, which would be copied whole
-// first (4 rows of 4095 x 16383 float16: 65 us, 101); one row of float16 (8192 x 8192 24.1 us here, 30.5 there; 4096 x 16384 23.5,
+// written by a pass of their own (4 rows: 47 us here, 200 there); weights that TMA cannot address, which would be copied whole
+// first (4 rows of 4095 x 16383 float16: 44 us, 101); one row of float16 (8192 x 8192 24.1 us here, 30.5 there; 4096 x 16384 23.5,
 // 26.7; 1000 x 50264 19.6, 25.0; 4096 x 1024 10.5, 10.0).  Two to eight rows of float16 are the tensor cores' (4 rows of the
 // 4096 x 16384: 48 us here, 26.7 there).
 // It also takes the small products of few rows that one 128 x 128 CUDA-core tile would walk alone (1024 x 1024, one row:
@@ -49,13 +49,15 @@ __device__ __forceinline__ void read_x(const float* xs, int k, float (&x)[kM]) {
 
 // w stored [K][N], from the CTA's first row and column on: a thread owns eight columns (adjacent where 16-byte loads allow it,
 // else 64 apart, so that a warp's loads are adjacent), four groups of 64 threads take every fourth of the `n` rows.
-template <typename T, int kM, bool kVec>
+template <typename T, int kM, bool kVec, bool kGroups>
 __device__ __forceinline__ void walk_columns(const T* w, int64_t ldw, int64_t cols, const float* xs, int n, float (&acc)[kM][8]) {
   const int tx = threadIdx.x % 64, ky = threadIdx.x / 64;
   w += kVec ? tx * 8 : tx;
-  // Rows whose loads are under way together; single elements of few rows want more of them (4095 x 16383 float16: one row 55.7 us with
-  // two, 38.5 with four; four rows 44.7, 55.9).
-  constexpr int kAhead = kVec ? (sizeof(T) == 2 ? 8 : 4) : kM <= 2 ? 4 : 2;
+  // Rows whose loads are under way together.  Single elements of few rows want more of them (4095 x 16383 float16: one row 55.7 us with
+  // two, 38.5 with four; four rows 44.7, 55.9); float32 chunks of three or four rows fewer, which lets a third CTA onto an SM (4096 x
+  // 16384, four rows: 55.9 us with four, 47.4 with two), and of more rows as many as fit two CTAs (eight rows: 63.6, 76.5), except
+  // beside the other forms of a kernel for groups, whose registers they set (64 groups of 1024 x 4096 over two rows: 232 us, 162).
+  constexpr int kAhead = kVec ? (sizeof(T) == 2 ? 8 : kM <= 2 || (kM > 4 && !kGroups) ? 4 : 2) : kM <= 2 ? 4 : 2;
   auto row = [&](int k, const float (&v)[8]) {
     float x[kM];
     read_x<kM>(xs, k, x);
@@ -238,7 +240,7 @@ __global__ void __launch_bounds__(256) skinny_columns_kernel(const SkinnyJob j) 
   __syncthreads();
   float acc[kM][8];
   clear(acc);
-  walk_columns<T, kM, kVec>((const T*)j.w + k0 * j.ldw + col0, j.ldw, j.N - col0, smem, n, acc);
+  walk_columns<T, kM, kVec, false>((const T*)j.w + k0 * j.ldw + col0, j.ldw, j.N - col0, smem, n, acc);
   join_columns<kM, kVec>(smem, acc, [&](int m, int c, float s) {
     if (col0 + c < j.N) j.ws[((int64_t)blockIdx.y * kM + m) * j.ws_ld + col0 + c] = s;
   });
@@ -405,7 +407,7 @@ __device__ __forceinline__ void few_tile(const FewJob& j, float* smem, int g, in
       __syncthreads();
       stage_x<T, kM, false>(smem, x + k0, j.inner, rows, n);
       __syncthreads();
-      walk_columns<T, kM, kVec>(w + k0 * j.cols + col0, j.cols, j.cols - col0, smem, n, acc);
+      walk_columns<T, kM, kVec, true>(w + k0 * j.cols + col0, j.cols, j.cols - col0, smem, n, acc);
     }
     join_columns<kM, kVec>(smem, acc, [&](int m, int c, float s) {
       if (m < rows && col0 + c < j.cols) out[m * j.cols + col0 + c] = narrow_f<T>(s);
@@ -524,8 +526,9 @@ cudaError_t launch_few_typed(const GroupedProblem& p, const GroupTiles& t, int64
   const bool vec = ((uintptr_t)p.b & 15) == 0 && ld % 8 == 0;
   FewJob j = {p.a, p.b, p.out, p.inner, p.cols, t, few_strips(p)};
   void* args[] = {(void*)&j};
-  const void* fn = p.trans_b ? (vec ? (const void*)few_rows_kernel<T, true, true> : (const void*)few_rows_kernel<T, false, true>)
-                             : (vec ? (const void*)few_rows_kernel<T, true, false> : (const void*)few_rows_kernel<T, false, false>);
+  const void* fn = p.trans_b ? (const void*)few_rows_kernel<T, false, true> : (const void*)few_rows_kernel<T, false, false>;
+  if constexpr (sizeof(T) == 4)   // float16 that 16-byte loads can read is the tensor cores'
+    if (vec) fn = p.trans_b ? (const void*)few_rows_kernel<T, true, true> : (const void*)few_rows_kernel<T, true, false>;
   return launch_behind(fn, args, dim3((unsigned)tiles), dim3(256), 49152, stream);   // eight staged rows; three groups' sums
 }
 
@@ -535,7 +538,7 @@ int few_strips(const GroupedProblem& p) { return (int)((p.cols + (p.trans_b ? 63
 
 // Groups of few rows, on the average (the offsets are not known to the host).  Forward: where the tensor cores would first have the
 // weights copied or split, which reads and writes them once more each (57 experts of 1049 x 2832 float32, two rows each:
-// 545 us there, 151 here); weight gradient: while a sum over the rows costs less than writing the result
+// 545 us there, 148 here); weight gradient: while a sum over the rows costs less than writing the result
 // (104 groups of 312 x 1251 float32 over nine rows in all: 331 us there, 34 here), but for float16 that TMA can address (64 groups of
 // 1024 x 4096 over two rows each: 128 us there, 150 here).
 bool few_preferred(const GroupedProblem& p) {
