@@ -116,7 +116,9 @@ class Experts:
 
 
 class AdamW:
-    """AdamW over the parameters of modules such as the above, one launch a step."""
+    """AdamW over the parameters of modules such as the above, one launch a step.  A module may replace a parameter's buffer between
+    steps (`layer.weight = ...`): the new one is trained from then on, with the moments that stood in its place.  Number and lengths of the
+    parameters are the first step's."""
 
     def __init__(self, backend: CUDABackend, modules: Sequence, learningRate: float = 1e-3, beta1: float = 0.9, beta2: float = 0.999,
                  epsilon: float = 1e-8, weightDecay: float = 0.01):
@@ -125,6 +127,7 @@ class AdamW:
         self.stepCount = 0
         self.plan: Optional[AdamWPlan] = None
         self.moments = []
+        self._planned = []   # the plan's parameters: (buffer, elements)
 
     def step(self) -> None:
         """Updates every parameter from its accumulated gradient; every parameter needs one."""
@@ -134,8 +137,16 @@ class AdamW:
             raise ValueError("AdamW: a parameter has no gradient")
         if self.plan is None:
             self.moments = [(be.constant(0.0, n, DType.float32), be.constant(0.0, n, DType.float32)) for _, _, n, _ in parameters]
+        elif len(parameters) != len(self._planned):
+            raise ValueError(f"AdamW: {len(parameters)} parameters, {len(self._planned)} at the first step")
+        else:
+            for i, ((_, _, n, _), (_, before)) in enumerate(zip(parameters, self._planned)):
+                if n != before:
+                    raise ValueError(f"AdamW: parameter {i} has {n} elements, {before} at the first step")
+        if self.plan is None or any(p is not q for (p, _, _, _), (q, _) in zip(parameters, self._planned)):
             self.plan = be.adamWPlan([dict(param=p, grad=g, moment1=m, moment2=v, count=n, dtype=t)
                                       for (p, g, n, t), (m, v) in zip(parameters, self.moments)])
+            self._planned = [(p, n) for p, _, n, _ in parameters]
         else:
             for i, (_, g, _, _) in enumerate(parameters):
                 self.plan.setGrad(i, g)
