@@ -181,6 +181,9 @@ hc_status run_grouped(hc_ctx* ctx, const hc::GroupedProblem& p) {
   const Span so = {p.out, no};
   if (overlap(so, {p.a, na}) || overlap(so, {p.b, nb}) || overlap(so, {p.offsets, (p.groups + 1) * 8}))
     return invalid(ctx, "the result overlaps another tensor");
+  // The table of groups and the tiles' coordinates are 32-bit, and a copy may start up to a tile behind the last row.
+  if (p.total_rows >= (1ll << 31) - 256)
+    return hc::ctx_fail(ctx, HC_ERR_NOT_IMPLEMENTED, "grouped product of 2^31 - 256 rows or more");
   if (p.weight_grad && p.total_rows == 0) {
     cudaError_t e = cudaMemsetAsync(p.out, 0, (size_t)no, hc::ctx_stream(ctx));
     return launched(ctx, e, 0, "grouped product");
