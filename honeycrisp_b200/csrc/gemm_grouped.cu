@@ -234,6 +234,9 @@ cudaError_t launch_grouped(const GroupedProblem& p, cudaStream_t stream, unsigne
   }
   // Result rows and columns of a group, and the contracted length: the group's rows for the weight gradient.
   const int64_t m = wg ? p.rows : p.total_rows, n = p.cols;
+  // Tile coordinates are 32-bit, and a tile may start within the last one of them.
+  constexpr int64_t kMost = (1ll << 31) - 256;
+  if (m >= kMost || n >= kMost || p.inner >= kMost || p.groups * BK >= kMost) return cudaErrorNotSupported;
   const int64_t mean_rows = (p.total_rows + p.groups - 1) / p.groups;
   Operand a = wg ? describe(p.a, 1, p.total_rows, p.rows, eb) : describe(p.a, 1, p.total_rows, p.inner, eb);
   Operand b = wg ? describe(p.b, 1, p.total_rows, p.cols, eb)
@@ -269,7 +272,7 @@ cudaError_t launch_grouped(const GroupedProblem& p, cudaStream_t stream, unsigne
   tp.tiles_m = wg ? (int)((m + tp.tile_rows - 1) / tp.tile_rows) : 1;
   const int64_t per_group = wg ? (int64_t)tp.tiles_m * tp.tiles_n : 0;
   tp.total_tiles = wg ? per_group * p.groups : (p.total_rows / tp.tile_rows + p.groups) * tp.tiles_n;   // forward: at most
-  if (tp.total_tiles >= (1ll << 31) || m >= (1ll << 31) - 256 || n >= (1ll << 31) - 256 || tail_rows >= (1ll << 31)) return cudaErrorNotSupported;
+  if (tp.total_tiles >= (1ll << 31)) return cudaErrorNotSupported;
 
   cudaError_t e = empty ? cudaSuccess : launch_operands(a, b, eb, stream, rec);
   if (e != cudaSuccess) return e;

@@ -23,3 +23,18 @@ def test_too_many_rows(rows, dtype):
     assert (matrices.onCPU(dtype)[:2] == 1).all()
     be.checkDeviceStatus()
     be.close()
+
+
+def test_too_long_a_contraction_for_tile_coordinates():
+    """One row of float16 and a matrix that lies as TMA needs it: the tensor cores' product, whose contracted index is a 32-bit coordinate."""
+    from honeycrisp_b200 import CUDABackend, NotImplementedByBackend
+    be = CUDABackend(0)
+    for inner in (2 ** 31, 2 ** 31 + 8):
+        x, matrix = be.allocate(inner * 2), be.allocate(inner * 2)
+        offsets, out = be.collection(np.array([0, 1]), np.int64), be.constant(1.0, 1, np.float16)
+        launches = be.launchCount()
+        with pytest.raises(NotImplementedByBackend, match="too large"):
+            be.groupedMatmul(1, offsets, x, matrix, True, 1, inner, 1, np.float16, out=out)
+        assert be.launchCount() == launches and out.onCPU(np.float16)[0] == 1
+    be.checkDeviceStatus()
+    be.close()
