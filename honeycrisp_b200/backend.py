@@ -282,6 +282,8 @@ class AdamWPlan:
                 if isinstance(x, np.ndarray):
                     raise TypeError(f"AdamWPlan: {name} must lie on the device")
                 ptr, keep = backend._input(x, dt, count, name)
+                if name != "grad":
+                    backend._own(x, name)
                 setattr(row, name, ptr or None)
                 if name == "grad":
                     self._grads[index] = keep
@@ -617,7 +619,8 @@ class CUDABackend:
     # Tensors of these calls are device buffers (CUDAData), contiguous CUDA torch tensors, or, for inputs,
     # numpy arrays, which are staged.  Sizes are checked here; what the library refuses (overlaps, misaligned
     # addresses, unknown activations, ranges of the scalars) raises ValueError.  Nothing here orders the backend's stream after
-    # torch's: run on torch's (useStream), or synchronise where tensors change hands and keep torch inputs alive until then.
+    # torch's or another backend's: run on torch's (useStream), or synchronise where tensors change hands and keep such inputs alive until
+    # then.  Results are this backend's own buffers or torch tensors.
 
     def _float_dtype(self, dtype, what: str):
         try:
@@ -661,6 +664,12 @@ class CUDABackend:
             raise ValueError(f"{what} is smaller than its {count} elements")
         return ptr, keep
 
+    def _own(self, x, what: str) -> None:
+        """Refuses a result buffer of another backend: its owner marks and frees it in the order of its own stream, so that wait() would
+        return, and its memory go, before this backend's stream has written it."""
+        if isinstance(x, CUDAData) and x.backend is not self:
+            raise ValueError(f"{what} belongs to another backend; wrap() it with this one, and order their streams")
+
     def _result(self, x, dt: DType, count: int, what: str):
         """(address, the result itself): `x`, or a fresh buffer where it is None."""
         if x is None:
@@ -668,6 +677,7 @@ class CUDABackend:
         elif isinstance(x, np.ndarray):
             raise TypeError(f"{what} must lie on the device")
         ptr, _ = self._input(x, dt, count, what)
+        self._own(x, what)
         return ptr, x
 
     def _done(self, results, inputs, mark: bool):
