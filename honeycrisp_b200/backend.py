@@ -809,7 +809,13 @@ class CUDABackend:
 
     def adamW(self, plan: "AdamWPlan", step: int, learningRate: float = 1e-3, beta1: float = 0.9, beta2: float = 0.999,
               epsilon: float = 1e-8, weightDecay: float = 0.01, mark: bool = True) -> None:
-        """One AdamW step over the plan's tensors, in place; `step` counts from 1."""
+        """One AdamW step over the plan's tensors, in place; `step` counts from 1.  A plan of torch tensors alone may run on any
+        backend of its device, one with CUDAData on the backend that laid it out."""
+        if plan._backend is not self:
+            if plan._backend.device != self.device:
+                raise ValueError(f"AdamW: the plan lies on device {plan._backend.device}, the backend on device {self.device}")
+            if plan._updated:
+                raise ValueError("AdamW: the plan's buffers belong to another backend")
         self._check(self._lib.hc_adamw(self._ctx, plan._table, plan.count, step, learningRate, beta1, beta2, epsilon, weightDecay))
         if mark:
             for t in plan._updated:

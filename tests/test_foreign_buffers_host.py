@@ -78,3 +78,20 @@ def test_a_plan_refuses_what_it_would_update_of_another_backend(be, beside, fiel
     with pytest.raises(ValueError, match="belongs to another backend"):
         be.adamWPlan([row(be), row(be, **{field: data(beside, 8, 4)})])
     be.adamWPlan([row(be, grad=data(beside, 8, 4))])   # read only
+
+
+def test_a_plan_of_another_backend_is_refused(be, beside):
+    plan = beside.adamWPlan([row(beside)])
+    with pytest.raises(ValueError, match="another backend"):
+        be.adamW(plan, 1)
+    assert not [n for n, _ in be._lib.calls if n == "hc_adamw"]
+    beside.adamW(plan, 1)
+    assert len([n for n, _ in beside._lib.calls if n == "hc_adamw"]) == 1
+
+
+def test_a_plan_of_another_device_is_refused(be):
+    far = backend(1)
+    plan = far.adamWPlan([])
+    with pytest.raises(ValueError, match="device 1"):
+        be.adamW(plan, 1)
+    far._ctx = None
