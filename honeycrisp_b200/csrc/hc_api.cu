@@ -26,8 +26,8 @@ struct hc_ctx {
   // Work area of the float32 split operands; grown on demand, freed with the context.
   void* scratch = nullptr;
   size_t scratch_bytes = 0;
-  // A captured graph keeps the address of the work area it was captured with: once one has used it, an
-  // outgrown area is kept until the context goes instead of being freed.
+  // A captured graph keeps the address of the work area it was captured with: an area that one has used
+  // is kept until the context goes instead of being freed when it is outgrown.
   bool scratch_in_graph = false;
   std::vector<void*> retired_scratch;
   // Device staging buffers of the host-buffer entry point.
@@ -170,7 +170,7 @@ hc_status ensure_scratch(hc_ctx* ctx, size_t need) {
   if (ctx->scratch) ctx->retired_scratch.push_back(ctx->scratch);
   ctx->scratch = fresh;
   ctx->scratch_bytes = need;
-  if (capturing) ctx->scratch_in_graph = true;
+  ctx->scratch_in_graph = capturing;   // of the fresh area: the one before is kept, this one only if a graph sees it
   return HC_OK;
 }
 

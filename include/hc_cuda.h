@@ -159,9 +159,9 @@ void hc_event_destroy(hc_event* ev);
  * largest need seen: the low TF32 halves of float32 operands, float16 operands repacked to an
  * aligned pitch, and at most 256 MiB of float32 partial sums when a long contraction over few
  * outputs is cut into parts); growing it is the only allocation a product makes, and it is
- * stream-ordered from the context's pool (no device-wide synchronisation).  A CUDA graph that
- * captured products is invalid once a later, larger product has grown the work area: run the
- * largest product once before capturing.  The context remembers how it prepared its most recent
+ * stream-ordered from the context's pool (no device-wide synchronisation).  An area that a captured
+ * CUDA graph has used is not freed when a later product outgrows it, so the graph stays valid.  The context
+ * remembers how it prepared its most recent
  * products (tile plan, tensor maps), so repeating a product on the same buffers costs the host
  * little more than the launch.  Results do not depend on how the work is tiled, cut or
  * scheduled: the same call gives the same bits.  Under HC_KERNEL_AUTO products too small for a
