@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(32 * kPartWarps) sum_parts_kernel(const PartsJ
     const int64_t pitch = j.M * j.ws_ld;
 #pragma unroll 4
     for (int z = warp; z < j.parts; z += warps) {
-      const float4 v = __ldg((const float4*)(src + z * pitch));
+      const float4 v = __ldcg((const float4*)(src + z * pitch));
       acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
     }
   }

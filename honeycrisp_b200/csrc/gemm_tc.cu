@@ -47,9 +47,9 @@ __global__ void __launch_bounds__(256) splitk_reduce_kernel(const ReduceJob j) {
     const int64_t g = i % groups, row = (i / groups) % j.M, mat = i / (groups * j.M);
     const int64_t n = g * 4;
     const float* src = j.ws + (mat * j.parts) * part_stride + row * j.ws_ld + n;
-    float4 acc = __ldg((const float4*)src);
+    float4 acc = __ldcg((const float4*)src);
     for (int z = 1; z < j.parts; z++) {
-      const float4 v = __ldg((const float4*)(src + z * part_stride));
+      const float4 v = __ldcg((const float4*)(src + z * part_stride));
       acc.x = __fadd_rn(acc.x, v.x); acc.y = __fadd_rn(acc.y, v.y);
       acc.z = __fadd_rn(acc.z, v.z); acc.w = __fadd_rn(acc.w, v.w);
     }
@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256) splitk_reduce_kernel(const ReduceJob j) {
       for (int e = 0; e < 4; e++) {
         h[e] = __float2half_rn(x[e]);
         if (j.bias && e < valid)
-          h[e] = __float2half_rn(__fadd_rn(__half2float(h[e]), __half2float(__ldg((const __half*)j.bias + n + e))));
+          h[e] = __float2half_rn(__fadd_rn(__half2float(h[e]), __half2float(((const __half*)j.bias)[n + e])));
       }
       __half* dst = (__half*)j.C + mat * j.strideC + row * j.ldc + n;
       if (valid == 4 && j.vec_ok) {
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(256) splitk_reduce_kernel(const ReduceJob j) {
       if (j.bias)
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          if (e < valid) x[e] = __fadd_rn(x[e], __ldg((const float*)j.bias + n + e));
+          if (e < valid) x[e] = __fadd_rn(x[e], ((const float*)j.bias)[n + e]);
       float* dst = (float*)j.C + mat * j.strideC + row * j.ldc + n;
       if (valid == 4 && j.vec_ok) {
         *(float4*)dst = make_float4(x[0], x[1], x[2], x[3]);

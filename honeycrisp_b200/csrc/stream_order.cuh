@@ -9,7 +9,9 @@ namespace hc {
 // stream is still draining.  `pdl_release` lets the successor be scheduled as soon as every CTA of this
 // grid has issued it (or exited); `pdl_wait` blocks until the predecessor has completed and its memory is
 // visible.  Both are no-ops for an ordinary launch.  Everything before pdl_wait must touch no global
-// memory that an earlier kernel may write.
+// memory that an earlier kernel may write.  Behind it, loads go by the coherent path: the non-coherent one
+// (the read-only cache) is for memory that does not change while the kernel runs, and the kernel may have
+// started while its predecessor was still writing.  Both cost the same here.
 __device__ __forceinline__ void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

@@ -440,7 +440,7 @@ __device__ __forceinline__ void add_bias(const void* bias, int64_t col, int64_t 
   if (kHalf) {
     const __half* b = (const __half*)bias + col;
     if (W == 8 && col + 8 <= N && (((uintptr_t)b) & 15) == 0) {
-      const uint4 u = __ldg((const uint4*)b);
+      const uint4 u = *(const uint4*)b;
       const __half2* h2 = (const __half2*)&u;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -451,17 +451,17 @@ __device__ __forceinline__ void add_bias(const void* bias, int64_t col, int64_t 
     } else {
 #pragma unroll
       for (int i = 0; i < W; i++)
-        if (col + i < N) x[i] = __fadd_rn(__half2float(__float2half_rn(x[i])), __half2float(__ldg(b + i)));
+        if (col + i < N) x[i] = __fadd_rn(__half2float(__float2half_rn(x[i])), __half2float(b[i]));
     }
   } else {
     const float* b = (const float*)bias + col;
     if (W == 4 && col + 4 <= N && (((uintptr_t)b) & 15) == 0) {
-      const float4 f = __ldg((const float4*)b);
+      const float4 f = *(const float4*)b;
       x[0] = __fadd_rn(x[0], f.x); x[1] = __fadd_rn(x[1], f.y); x[2] = __fadd_rn(x[2], f.z); x[3] = __fadd_rn(x[3], f.w);
     } else {
 #pragma unroll
       for (int i = 0; i < W; i++)
-        if (col + i < N) x[i] = __fadd_rn(x[i], __ldg(b + i));
+        if (col + i < N) x[i] = __fadd_rn(x[i], b[i]);
     }
   }
 }
@@ -1198,7 +1198,7 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
                 if (kCode < kGradCode && p.fe.bias) {
                   const __half* b = (const __half*)p.fe.bias + col0 + k;
                   if (cols_here >= k + W && ((uintptr_t)b & 15) == 0) {
-                    Pack16<__half>::widen(__ldg((const uint4*)b), bias);
+                    Pack16<__half>::widen(*(const uint4*)b, bias);
                   } else {
 #pragma unroll
                     for (int e = 0; e < W; e++) bias[e] = k + e < cols_here ? __half2float(b[e]) : 0.0f;
@@ -1479,7 +1479,7 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap mapA_hi, const __grid_constan
                 for (int e = 0; e < 4; e++) {
                   x[e] = acc[c + q * 4 + e];
                   aux[e] = 0.0f;
-                  bias[e] = kCode < kGradCode && p.fe.bias && q * 4 + e < cols_here ? __ldg((const float*)p.fe.bias + n0 + c + q * 4 + e) : 0.0f;
+                  bias[e] = kCode < kGradCode && p.fe.bias && q * 4 + e < cols_here ? ((const float*)p.fe.bias)[n0 + c + q * 4 + e] : 0.0f;
                 }
                 if (p.fe.aux) Pack16<float>::widen(ld_shared_v4(own_row + (((uint32_t)q ^ sw) << 4)), aux);
                 fused_values<kCode, false, 4>(x, bias, aux, zq);
