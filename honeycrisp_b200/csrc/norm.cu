@@ -281,7 +281,8 @@ __global__ void __launch_bounds__(kThreads* kRows, kThreads* kRows <= 512 ? 2 : 
 // walks its rows, kBatch of them at a time: one round of sums, whose latency no other work of the CTA hides, serves them all.
 // At the end each CTA leaves one row of the partial matrices [2][CTAs][cols], which sum_runs_kernel adds in order.  The grid,
 // and so the order of the sums, depends on shape, alignment and device alone.
-// h is x rstd - mean rstd, one multiply-add an element: off by 2^-24 |mean| rstd at most, which the mean's own rounding is too.
+// h is (x - mean) rstd, the difference first: x rstd - mean rstd, one instruction for a pair where this takes two, is off by 2^-24 |mean| rstd,
+// which on rows whose mean is thousands of times their spread is thousands of times the rounding of h.
 template <typename T, int kW, int kC, int kThreads, int kRows, int kBatch>
 struct BackwardLayout {
   static constexpr int kBatches = queue_batches(2 * kBatch * kThreads * kRows * kC * 16, kThreads * kRows > 256 ? 131072 : 65536);   // 128 KB an SM
@@ -364,11 +365,11 @@ __global__ void __launch_bounds__(kThreads* kRows, kThreads * kRows <= 256 ? 2 :
 #pragma unroll
     for (int r = 0; r < kBatch; r++) {
       rstd[r] = rstd_at[r];
-      const float2 scale = both(rstd[r]), off = both(-mean_at[r] * rstd[r]);
+      const float2 scale = both(rstd[r]), off = both(-mean_at[r]);
       float2 s0 = both(0.0f), s1 = both(0.0f);
 #pragma unroll
       for (int e = 0; e < P; e++) {
-        h[r][e] = fma2(h[r][e], scale, off);   // past the row's end g is zero, and so is all that follows from it
+        h[r][e] = mul2(add2(h[r][e], off), scale);   // past the row's end g is zero, and so is all that follows from it
         db[e] = add2(db[e], g[r][e]);
         dw[e] = fma2(g[r][e], h[r][e], dw[e]);
         g[r][e] = mul2(g[r][e], w[e]);
