@@ -320,10 +320,13 @@ struct TcPrepared {
 
 // What the tensor-core kernel most recently launched on a stream wrote.  Consulted only for
 // streams the library owns (nobody else enqueues kernels there), where it decides whether the
-// next kernel's operand loads may run ahead of the wait for its predecessor.
+// next kernel's operand loads may run ahead of the wait for its predecessor.  A launch that was captured
+// into a graph is a predecessor to launches of the same capture only: it has not run, and what is
+// launched next on the stream follows what was launched before the capture.
 struct StreamTrack {
   cudaStream_t stream = nullptr;
   bool used = false, known = false;
+  unsigned long long capture = 0;   // 0: launched, else the capture's id
   uintptr_t lo = 0, hi = 0;
   uint64_t stamp = 0;
 };
@@ -656,14 +659,20 @@ cudaError_t issue_tc(const TcPrepared& pp, int sm_count, cudaStream_t stream, La
   // starts at all.)
   bool skip = false;
   if (private_stream && overlap_launches()) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long capture = 0;
+    const bool told = cudaStreamGetCaptureInfo(stream, &status, &capture) == cudaSuccess;
+    if (!told) cudaGetLastError();
+    if (status == cudaStreamCaptureStatusNone) capture = 0;
     std::lock_guard<std::mutex> lock(g_track_mu);
     StreamTrack* t = track_entry(stream, true);
-    if (t->known && pp.trackable) {
+    if (t->known && told && t->capture == capture && pp.trackable) {
       skip = true;
       for (int i = 0; i < 3; i++)
         if (pp.in_hi[i] > pp.in_lo[i] && pp.in_lo[i] < t->hi && t->lo < pp.in_hi[i]) skip = false;
     }
-    t->known = pp.trackable;
+    t->known = pp.trackable && told;
+    t->capture = capture;
     t->lo = pp.out_lo;
     t->hi = pp.out_hi;
     t->stamp = ++g_track_clock;
