@@ -646,6 +646,8 @@ class CUDABackend:
                 raise ValueError(f"{what} is smaller than its {count} elements")
             if x.backend is not self and x.backend.device != self.device:
                 raise ValueError(f"{what} lies on device {x.backend.device}, the backend on device {self.device}")
+            if not x.ptr and count > 0:   # null would read as an optional tensor that was not given
+                raise ValueError(f"{what} has been freed")
             return x.ptr, x
         if hasattr(x, "element_size"):   # a torch tensor
             if _TORCH_DTYPE.get(x.dtype) is not dt and _torch_dtype(x.dtype) is not dt:
@@ -674,7 +676,8 @@ class CUDABackend:
         """(address, the result itself): `x`, or a fresh buffer where it is None."""
         if x is None:
             x = self.allocate(count * dt.byteSize)
-        elif isinstance(x, np.ndarray):
+            return x.ptr, x
+        if isinstance(x, np.ndarray):
             raise TypeError(f"{what} must lie on the device")
         ptr, _ = self._input(x, dt, count, what)
         self._own(x, what)
