@@ -150,8 +150,8 @@ class AdamW:
         else:
             for i, (_, g, _, _) in enumerate(parameters):
                 self.plan.setGrad(i, g)
+        be.adamW(self.plan, self.stepCount + 1, **self.hyper)
         self.stepCount += 1
-        be.adamW(self.plan, self.stepCount, **self.hyper)
 
     def zeroGrad(self) -> None:
         for m in self.modules:

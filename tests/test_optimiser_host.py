@@ -77,3 +77,18 @@ def test_other_parameters_than_the_first_steps_are_refused(be):
     with pytest.raises(ValueError, match="elements"):
         optimiser.step()
     assert len(steps(be)) == 1
+
+
+def test_a_step_that_failed_does_not_count(be):
+    m = Module(be, 40)
+    optimiser = AdamW(be, [m])
+    optimiser.step()
+    optimiser.hyper["epsilon"], good = -1.0, optimiser.hyper["epsilon"]
+    refuse = lambda *a: L.HC_ERR_INVALID_ARGUMENT if a[7] < 0 else L.HC_OK  # noqa: E731
+    be._lib.hc_adamw, be._lib.hc_last_error = refuse, lambda *a: b"epsilon must not be negative"
+    with pytest.raises(ValueError, match="epsilon"):
+        optimiser.step()
+    optimiser.hyper["epsilon"] = good
+    del be._lib.hc_adamw
+    optimiser.step()
+    assert [args[3] for name, args, _ in be._lib.calls if name == "hc_adamw"] == [1, 2] and optimiser.stepCount == 2
