@@ -164,7 +164,7 @@ const void* kernel_of(bool vec, bool sum) {
 }
 template <typename T>
 cudaError_t launch_typed(const void* grad, const void* pre, int64_t rows, int64_t cols, void* dpre, float* bias_grad,
-                         float* partial, bool vec, const RunSplit& s, int act, cudaStream_t stream) {
+                         float* partial, bool vec, const RunSplit& s, int act, int* launches, cudaStream_t stream) {
   const void* fn = nullptr;
   switch (act) {
     case HC_ACT_RELU: fn = kernel_of<T, HC_ACT_RELU>(vec, bias_grad); break;
@@ -176,7 +176,10 @@ cudaError_t launch_typed(const void* grad, const void* pre, int64_t rows, int64_
   int64_t per = s.rows_per_run;
   void* args[] = {(void*)&grad, (void*)&pre, (void*)&dpre, (void*)&partial, (void*)&rows, (void*)&cols, (void*)&per};
   cudaError_t e = launch_behind(fn, args, dim3((unsigned)s.strips, (unsigned)s.runs), dim3(kLanes * kWarps), 0, stream);
-  if (e != cudaSuccess || !bias_grad || s.runs == 1) return e;   // one run's partial matrix is the sum
+  if (e != cudaSuccess) return e;
+  *launches = 1;
+  if (!bias_grad || s.runs == 1) return e;   // one run's partial matrix is the sum
+  *launches = 2;
   return launch_sum_runs(partial, s.runs, cols, bias_grad, nullptr, false, stream);
 }
 bool rows_of_16_bytes(const void* a, const void* b, const void* c, int64_t row_bytes) {
@@ -191,14 +194,15 @@ size_t activation_grad_scratch(hc_dtype dtype, int64_t rows, int64_t cols) {
 }
 
 cudaError_t launch_activation_grad(hc_dtype dtype, int act, const void* grad, const void* pre, int64_t rows, int64_t cols,
-                                   void* dpre, float* bias_grad, float* scratch, cudaStream_t stream) {
+                                   void* dpre, float* bias_grad, float* scratch, int* launches, cudaStream_t stream) {
+  *launches = 0;
   const int64_t eb = dtype == HC_F16 ? 2 : 4;
   const bool vec = rows_of_16_bytes(grad, pre, dpre, cols * eb);
   const RunSplit s = split_runs(rows, cols, kLanes * (vec ? (int)(16 / eb) : 1));
   if (s.strips > 2147483647LL || s.runs > 65535) return cudaErrorInvalidValue;
   if (s.runs == 1) scratch = bias_grad;
-  return dtype == HC_F16 ? launch_typed<__half>(grad, pre, rows, cols, dpre, bias_grad, scratch, vec, s, act, stream)
-                         : launch_typed<float>(grad, pre, rows, cols, dpre, bias_grad, scratch, vec, s, act, stream);
+  return dtype == HC_F16 ? launch_typed<__half>(grad, pre, rows, cols, dpre, bias_grad, scratch, vec, s, act, launches, stream)
+                         : launch_typed<float>(grad, pre, rows, cols, dpre, bias_grad, scratch, vec, s, act, launches, stream);
 }
 
 }  // namespace hc

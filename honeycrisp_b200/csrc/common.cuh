@@ -159,7 +159,7 @@ RunSplit split_runs(int64_t rows, int64_t cols, int cols_per_cta);
 cudaError_t launch_sum_runs(const float* partial, int64_t runs, int64_t cols, void* out0, void* out1, bool half, cudaStream_t stream);
 size_t activation_grad_scratch(hc_dtype dtype, int64_t rows, int64_t cols);
 cudaError_t launch_activation_grad(hc_dtype dtype, int act, const void* grad, const void* pre, int64_t rows, int64_t cols,
-                                   void* dpre, float* bias_grad, float* scratch, cudaStream_t stream);
+                                   void* dpre, float* bias_grad, float* scratch, int* launches, cudaStream_t stream);
 cudaError_t launch_layer_norm(hc_dtype dtype, hc_dtype param_dtype, const void* x, const void* w, const void* b, int64_t rows,
                               int64_t cols, float epsilon, void* out, float* mean, float* rstd, int sm_count, cudaStream_t stream);
 size_t layer_norm_grad_scratch(hc_dtype dtype, int64_t rows, int64_t cols, int sm_count);

@@ -97,9 +97,10 @@ hc_status hc_activation_grad(hc_ctx* ctx, hc_dtype dtype, int activation, const 
     hc_status s = hc::ctx_scratch(ctx, hc::activation_grad_scratch(dtype, rows, cols), &scratch);
     if (s != HC_OK) return s;
   }
-  cudaError_t e = hc::launch_activation_grad(dtype, activation, grad, pre, rows, cols, dpre, bias_grad, (float*)scratch,
+  int launches = 0;
+  cudaError_t e = hc::launch_activation_grad(dtype, activation, grad, pre, rows, cols, dpre, bias_grad, (float*)scratch, &launches,
                                              hc::ctx_stream(ctx));
-  return launched(ctx, e, bias_grad ? 2 : 1, "activation gradient");
+  return launched(ctx, e, launches, "activation gradient");
 }
 
 hc_status hc_layer_norm(hc_ctx* ctx, hc_dtype dtype, hc_dtype param_dtype, const void* x, const void* weight, const void* bias,

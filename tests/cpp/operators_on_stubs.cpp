@@ -34,7 +34,7 @@ hc_status ctx_run_problem(hc_ctx*, const GemmProblem&, int64_t) { enqueued++; re
 cudaError_t launch_grouped(const GroupedProblem&, cudaStream_t, unsigned int*, void*, size_t, int, LaunchRecord*, size_t*) { enqueued++; return cudaSuccess; }
 size_t activation_grad_scratch(hc_dtype, int64_t, int64_t) { return 1; }
 size_t layer_norm_grad_scratch(hc_dtype, int64_t, int64_t, int) { return 1; }
-cudaError_t launch_activation_grad(hc_dtype, int, const void*, const void*, int64_t, int64_t, void*, float*, float*, cudaStream_t) { enqueued++; return cudaSuccess; }
+cudaError_t launch_activation_grad(hc_dtype, int, const void*, const void*, int64_t, int64_t, void*, float*, float*, int*, cudaStream_t) { enqueued++; return cudaSuccess; }
 cudaError_t launch_layer_norm(hc_dtype, hc_dtype, const void*, const void*, const void*, int64_t, int64_t, float, void*, float*, float*, int, cudaStream_t) { enqueued++; return cudaSuccess; }
 cudaError_t launch_layer_norm_grad(hc_dtype, hc_dtype, const void*, const void*, const void*, const float*, const float*, int64_t, int64_t, void*, void*, void*, float*, int, int*, cudaStream_t) { enqueued++; return cudaSuccess; }
 cudaError_t launch_adamw(const hc_adamw_tensor*, int64_t, const AdamWFactors&, int*, cudaStream_t) { enqueued++; return cudaSuccess; }
