@@ -10,9 +10,9 @@ import numpy as np
 
 HALF_STEP = {np.float16: 2.0 ** -11, np.float32: 2.0 ** -24}
 SMALLEST = {np.float16: 2.0 ** -25, np.float32: 2.0 ** -126}   # half a step of float16's subnormals; float32 may flush
-# float16 results take a polynomial of relative error 4.7e-6 and the hardware's exponential (2 + 1.2 |t| steps of 2^-23
-# for e^t, |t| < 90 where the value is not yet below float16's range); float32 ones 1.5e-7 and the exponent's rounding,
-# z^2 / 2 * 2^-23 with z <= 14.
+# Both types take the same fit, off by 1.7e-7.  float16 results take the hardware's exponential (2 + 1.2 |t| steps of 2^-23
+# for e^t, |t| < 90 where the value is not yet below float16's range).  For float32 this is the exponent's rounding at its
+# largest, z^2 / 2 * 2^-23 with z <= 14, wherever z lies; test_activation_accuracy_gpu.py has the room by z.
 ACT_RELATIVE = {np.float16: 2.0e-5, np.float32: 1.5e-5}
 
 _erfc = np.vectorize(math.erfc, otypes=[np.float64])
