@@ -188,7 +188,7 @@ bool rows_of_16_bytes(const void* a, const void* b, const void* c, int64_t row_b
 }  // namespace
 
 size_t activation_grad_scratch(hc_dtype dtype, int64_t rows, int64_t cols) {
-  // the wider split's matrix fits the narrower one's count of runs too: one column a lane gives the fewest runs
+  // alignment decides between a 16-byte chunk and one column a lane, and with it the split: room for either
   const RunSplit v = split_runs(rows, cols, kLanes * (dtype == HC_F16 ? 8 : 4)), n = split_runs(rows, cols, kLanes);
   return (size_t)(v.runs > n.runs ? v.runs : n.runs) * (size_t)cols * 4;
 }

@@ -75,7 +75,7 @@ __device__ __forceinline__ void store_four(void* p, int half, int64_t k, const f
 }
 
 // A CTA updates kChunk elements of one tensor.  All of a thread's quads are read before the first is written, which
-// keeps 16 loads of 16 bytes in flight; the few elements around the aligned quads go one by one.
+// keeps eight loads in flight, of 16 bytes each (8 of float16); the few elements around the aligned quads go one by one.
 template <int kMax>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ AdamJob<kMax> j) {
   int lo = 0, hi = j.n - 1;

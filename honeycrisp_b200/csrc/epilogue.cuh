@@ -23,7 +23,7 @@ namespace hc {
 //
 // Phi(-y) = e^(-y^2/2) Q(y) for y >= 0 and Phi(y) = 1 - Phi(-y), where Q falls slowly from 1/2 and is fitted
 // by t R(t), t = 1/(1 + 0.3 y), R a polynomial of degree 7, with least largest relative error over y <= 14 (Phi(-14) is 8e-45,
-// below float32's normals): 1.5e-7.  The exponent's rounding dominates: 6e-7 of Phi at z = -3, 1.3e-6 at -6.
+// below float32's normals): 1.7e-7.  The exponent's rounding dominates: 6e-7 of Phi at z = -3, 1.3e-6 at -6.
 // kFast, for float16 results, takes the hardware's exponential and reciprocal (a few 2^-23).
 __device__ __forceinline__ float exp2_approx(float t) {
   float r;

@@ -32,8 +32,8 @@ __device__ __forceinline__ float param_at(const void* p, int64_t c, int half) {
 
 // kN sums at once over the kThreads of a row (a warp, or several whole ones); every thread of the row gets them all.  The
 // butterfly halves the values while it halves the lanes (a lane keeps one half and sends the other), so that eight sums
-// take nine shuffles, not forty; lane i * 32 / kN ends with sum i.  `slot` alternates between successive calls, so that
-// one barrier each is enough; with more than one row group a CTA (kRows), each has a named barrier of its own.
+// take nine shuffles, not forty; lane i * 32 / kN ends with sum i, and a shuffle for each sum hands them to all.  `slot` alternates
+// between successive calls, so that one barrier each is enough; with more than one row group a CTA (kRows), each has a named barrier of its own.
 template <int kThreads, int kRows, int kN>
 __device__ __forceinline__ void row_sum(float (&v)[kN], float (*scratch)[kN][32], int& slot) {
   constexpr int kShare = 32 / kN;   // lanes that end with the same sum

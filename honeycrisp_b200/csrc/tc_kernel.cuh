@@ -655,8 +655,8 @@ __device__ __forceinline__ KRange k_range(int64_t vmat, const TcParams& p) {
 //             unrounded product instead of the bias of Linear to the rounded one;
 //             kGrouped: products grouped by expert (TcParams::groups).  Forward, A's rows are one tall matrix
 //             and B holds one matrix a group: a tile loads past its group's end (the neighbour's rows land in
-//             accumulator rows that are never stored), and a warp whose 32 rows reach past it stores from
-//             registers.  Weight gradient, the group's rows are contracted: whole slabs come from the
+//             accumulator rows that are never stored), and a warp whose 32 rows reach past it stores
+//             them a row at a time.  Weight gradient, the group's rows are contracted: whole slabs come from the
 //             operands, the last partial one from a zero-padded copy (maps 1.. of `mapC`), because rows of the
 //             neighbour would be summed; a group without rows gets zeros.
 // One CTA per SM: a kernel that allocates tensor memory (tcgen05.alloc) is never given a second
