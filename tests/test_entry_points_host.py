@@ -20,7 +20,7 @@ def lib(tmp_path_factory):
     if not os.path.exists(include) or shutil.which("g++") is None:
         pytest.skip("no host compiler or CUDA headers")
     path = str(tmp_path_factory.mktemp("stubs") / "operators.so")
-    subprocess.check_call(["g++", "-std=c++17", "-w", "-shared", "-fPIC", "-I", include, "-o", path, "-x", "c++", os.path.join(ROOT, "tests", "cpp", "operators_on_stubs.cpp"),
+    subprocess.check_call(["g++", "-std=c++17", "-w", "-shared", "-fPIC", "-Wl,-Bsymbolic", "-I", include, "-o", path, "-x", "c++", os.path.join(ROOT, "tests", "cpp", "operators_on_stubs.cpp"),
                            "-x", "c++", os.path.join(ROOT, "honeycrisp_b200", "csrc", "hc_ops.cu")])
     lib = ctypes.CDLL(path)
     for name, (res, args) in L.SIGNATURES.items():
