@@ -236,7 +236,7 @@ cudaError_t launch_grouped(const GroupedProblem& p, cudaStream_t stream, unsigne
   const int64_t m = wg ? p.rows : p.total_rows, n = p.cols;
   // Tile coordinates are 32-bit, and a tile may start within the last one of them.
   constexpr int64_t kMost = (1ll << 31) - 256;
-  if (m >= kMost || n >= kMost || p.inner >= kMost || p.groups * BK >= kMost) return cudaErrorNotSupported;
+  if (m >= kMost || n >= kMost || p.inner >= kMost) return cudaErrorNotSupported;
   const int64_t mean_rows = (p.total_rows + p.groups - 1) / p.groups;
   Operand a = wg ? describe(p.a, 1, p.total_rows, p.rows, eb) : describe(p.a, 1, p.total_rows, p.inner, eb);
   Operand b = wg ? describe(p.b, 1, p.total_rows, p.cols, eb)
