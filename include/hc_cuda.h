@@ -294,8 +294,7 @@ hc_status hc_layer_norm_grad(hc_ctx* ctx, hc_dtype dtype, hc_dtype param_dtype, 
  * before offsets[0] and from offsets[group_count] on are left as they are.  Offsets outside
  * [0, total_rows] or running backwards are clamped to stay in range and ascending.  `total_rows` is below
  * 2^31 - 256 (else HC_ERR_NOT_IMPLEMENTED), and so are the other lengths where the tensor cores take the
- * product.  With trans_b this is
- * also the gradient of the rows: d(a) = d(out) * b[g]^T.
+ * product; `group_count` is at most 65535.  With trans_b this is also the gradient of the rows: d(a) = d(out) * b[g]^T.
  * Next to: Backend.batchedMatmul (Backend.swift:661-669), whose matrices all have the same shape. */
 hc_status hc_grouped_matmul(hc_ctx* ctx, hc_dtype dtype, int64_t group_count,
                             const int64_t* offsets, const void* a, const void* b, int trans_b,
